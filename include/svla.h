@@ -68,6 +68,11 @@ typedef void* svla_stream_t; /* hipStream_t */
 #define SVLA_MASK_CAUSAL 1
 #define SVLA_MASK_PREFIX_LM 2
 
+/* Element formats of a K/V cache (svla_kv_*): blocks of 32 values of a row
+ * share a power of two. */
+#define SVLA_KV_MXFP4 4 /* e2m1 elements, 68 bytes a token and head (K and V) */
+#define SVLA_KV_MXFP8 8 /* e4m3 elements, 132 bytes */
+
 /* Layout flags of svla_linear_wide_bf16: slab-blocked A, W or C.  A blocked
  * [rows, K] matrix stores element (r, k) at (k / 32) * rows * 32 + r * 32 + k % 32. */
 #define SVLA_LAYOUT_A_BLOCKED 1
@@ -522,6 +527,86 @@ int svla_time_embedding_bf16(double t, int dim, double min_period, double max_pe
 
 /* fp32 -> bf16 conversion (round to nearest even), n values. */
 int svla_f32_to_bf16(const float* x, void* y, long n, svla_stream_t stream);
+
+/* svla_attention_bf16 with a sliding window and sinks: the query row r is at
+ * position q_pos + r, key j at position j; a row sees the keys j <= its
+ * position that are > position - window or < sinks, and < lens[b] (device
+ * int32 per sequence, clamped to [0, sk]; NULL: sk).  A row that sees nothing
+ * gives zeros, and no key that a row does not see reaches it, be it infinite
+ * or NaN.  window >= 1, sinks >= 0, q_pos >= 0, scale > 0. */
+int svla_attention_window_bf16(const void* q, int ldq, long q_bs, const void* k, int ldk, long k_bs,
+                               const void* v, int ldv, long v_bs, void* o, int ldo, long o_bs,
+                               int batch, int sq, int sk, int hq, int hkv, int head_dim,
+                               float scale, int q_pos, const int* lens, int window, int sinks,
+                               svla_stream_t stream);
+
+/* ------------------------------------------------------------- K/V cache --
+ * A cache of K and V in microscaled 8 or 4 bits.  No counterpart in the
+ * reference, which recomputes its whole prefix for every chunk
+ * (vla/vla.py:194-212).
+ *
+ * Sequence b holds the positions 0 .. n-1 of which, once n > sinks + ring, only
+ * the first `sinks` and the last (at least ring - 31) are kept: the ring is a
+ * whole number of 32-token records.  data: svla_kv_cache_bytes bytes, 16-byte
+ * aligned, zeroed once before the first use (a record may be decoded before
+ * every token of it was written).  state: [batch][2] int32, set by
+ * svla_kv_reset; state[b][0] is n.
+ *
+ * Values: 32 consecutive values of a row share a power of two 2^E, E in
+ * [-110, 126] the smallest for which none saturates (max|x| <= 6 2^E for e2m1,
+ * 448 2^E for e4m3); each is the nearest element, ties to the even code.
+ * Magnitudes over 1.5 2^127 are stored as that; a block that holds an infinity
+ * or a NaN reads as NaN throughout.
+ *
+ * One writer at a time: an append (svla_kv_append_bf16, svla_kv_reset) must not
+ * overlap with another call on the same cache; reads and attention may overlap
+ * with each other. */
+typedef struct {
+  void* data;
+  int* state;
+  int batch, n_kv_heads, head_dim; /* head_dim 64; batch * n_kv_heads <= 65535 */
+  int format;                      /* SVLA_KV_* */
+  int sinks;                       /* first positions that are always kept, >= 0 */
+  int ring;                        /* tokens of the ring, a multiple of 32 */
+} svla_kv_cache;
+
+/* Bytes of `data`; 0: not a valid cache. */
+long svla_kv_cache_bytes(int batch, int n_kv_heads, int head_dim, int format, int sinks, int ring);
+
+/* Every sequence empty. */
+int svla_kv_reset(const svla_kv_cache* c, svla_stream_t stream);
+
+/* Row r of sequence b (k + b*k_bs + r*ldk, heads side by side) is quantised
+ * into position p + r, p = at[b] or, with at NULL, the n tokens held; n becomes
+ * p + counts[b] (counts NULL: rows).  Rows behind counts[b] are not read;
+ * counts are clamped to [0, rows].  at[b] < n takes the later tokens back
+ * (those that have left the ring meanwhile stay lost); at[b] > n, at[b] < 0 or
+ * a position past 2^30 marks the sequence as lost: attention over it gives
+ * NaN and reading it zeros until it is written from position 0.  16-byte
+ * aligned rows, ld and batch strides % 8 == 0. */
+int svla_kv_append_bf16(const svla_kv_cache* c, const void* k, int ldk, long k_bs, const void* v,
+                        int ldv, long v_bs, int rows, const int* counts, const int* at,
+                        svla_stream_t stream);
+
+/* Rows start[b] .. start[b] + rows - 1 as bf16 (exactly the stored values);
+ * starts NULL: `start` for every sequence.  Positions that are not held are
+ * zeros. */
+int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void* v, int ldv,
+                      long v_bs, int start, const int* starts, int rows, svla_stream_t stream);
+
+/* Attention of the last counts[b] (NULL: rows) tokens of every sequence over
+ * it: query row r is at position p = n - counts[b] + r and sees the positions
+ * <= p, with window > 0 only those > p - window or < sinks.  Query head h reads
+ * KV head h * n_kv_heads / hq.  Scores, statistics and sums fp32,
+ * probabilities bf16, bf16 out.  Rows behind counts[b] are written as zeros.  A
+ * sequence of which a position that the call needs has left the ring (or that
+ * is lost, or holds fewer tokens than counts[b]) gives NaN.  scale > 0,
+ * rows * hq <= 2^24.  scratch: svla_kv_attention_scratch bytes, 4-byte aligned,
+ * of this call alone until it is done (NULL where that is 0). */
+long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window);
+int svla_kv_attention_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o,
+                           int ldo, long o_bs, int rows, const int* counts, int hq, float scale,
+                           int window, void* scratch, long scratch_bytes, svla_stream_t stream);
 
 /* ------------------------------------------------------- pre-processing --
  * Camera frames -> vision-encoder input: n uint8 RGB frames [h, w, 3]

@@ -1,0 +1,881 @@
+// K/V cache held in microscaled 8 or 4 bits: writing it, reading it back and
+// attention over it (gfx950, head_dim 64).
+//
+// Quantisation.  32 consecutive values of a row share a power of two 2^E; an
+// element is the nearest e4m3 or e2m1 number to x / 2^E (ties to the even
+// code: the rounding of v_cvt_scalef32_pk_{fp8,fp4}_bf16).  E is the smallest
+// exponent for which no element saturates, max|x| <= 448 2^E (6 2^E), held
+// within [-110, 126] as the byte E + 127.  With that range every stored value
+// is a normal bf16 number or zero, so reading back and the products below use
+// exactly the stored value.  Magnitudes over 1.5 2^127 are stored as that (the
+// next e2m1 step would be infinite).  A block that holds an infinity or a NaN
+// gets the scale byte 0xff and zero codes and reads as NaN throughout.
+//
+// Layout.  A record holds 32 tokens of one head of one sequence in the order
+// in which the attention's MFMAs take them, so that a wave reads it as whole
+// consecutive kilobytes, straight into operand registers:
+//   K (A operand of S^T = K . Q^T): lane (g, s & 15), g = lane / 16, holds for
+//     token half s >> 4 and depth half ks the codes of d = 32 ks + 8 g + 0..7;
+//     4 bits: one dword [half][ks] of the lane's 16 bytes; 8 bits: two dwords
+//     at [half] kilobyte, [ks] half of the lane's 16 bytes.
+//   V (A operand of O^T = V^T . P^T): lane (g, d & 15) holds for td = d >> 4
+//     the codes of the tokens 4 g + 0..3 and 16 + 4 g + 0..3 (the order in
+//     which S^T's accumulators become the operand P^T); 4 bits: dword [td];
+//     8 bits: [td >> 1] kilobyte, [td & 1] half.
+//   K scales: byte [s & 15][half][ks]; V scales: byte [g][d >> 5][8 tokens].
+// 4 bits: 1024 + 1024 + 64 + 64 bytes; 8 bits: 2048 + 2048 + 64 + 64.
+//
+// Positions.  The first `sinks` positions have records of their own; position
+// p >= sinks is token (p - sinks) % 32 of ring tile u = (p - sinks) / 32, held
+// in record u % (ring / 32) after the sinks'.  Per sequence the state is the
+// number of tokens n and the first ring tile still held, lo; lo = kLost marks
+// a sequence whose contents cannot be vouched for (a position that skips
+// ahead was written), until it is written from position 0 again.
+#include "attention_tile.h"
+
+namespace {
+
+constexpr int TOK = 32;                 // tokens of a record
+constexpr int kMaxPos = 1 << 30;        // positions stay below it
+constexpr int kLost = 0x7fffffff;
+
+template <int BITS> constexpr int kPart = TOK * D * BITS / 8;      // bytes of K (or V) codes
+template <int BITS> constexpr int kRec = 2 * kPart<BITS> + 128;
+
+struct Cache {
+  uint8_t* data;
+  int* state;                           // [batch][2]: n, lo
+  int heads, sinks, sink_tiles, ring_tiles;
+};
+
+__device__ __forceinline__ long record(const Cache& c, int b, int h, int tile) {
+  return ((long)b * c.heads + h) * (c.sink_tiles + c.ring_tiles) + tile;
+}
+
+// What a write of `count` rows at position p0 does to a sequence.
+struct Span {
+  int p0, n, lo;                        // first position, tokens and lo afterwards
+};
+__device__ __forceinline__ Span write_span(const Cache& c, int n, int lo, int p0, int count) {
+  Span s;
+  s.p0 = p0;
+  if (p0 < 0 || p0 > n || p0 > kMaxPos - count || (lo == kLost && p0 != 0)) {
+    s.n = n;
+    s.lo = kLost;
+    return s;
+  }
+  s.n = p0 + count;
+  // nothing of the ring is kept when the write begins inside the sinks
+  const int keep = p0 <= c.sinks ? 0 : lo;
+  const int last = s.n > c.sinks ? (s.n - 1 - c.sinks) >> 5 : -1;
+  s.lo = max(keep, last - c.ring_tiles + 1);
+  return s;
+}
+
+// The records that hold positions [p0, n): first the sinks', then the ring's
+// from tile u0.
+struct Tiles {
+  int s0, ns, u0, nr;
+};
+__device__ __forceinline__ Tiles tiles_of(const Cache& c, int p0, int n) {
+  Tiles t = {0, 0, 0, 0};
+  if (p0 >= n) return t;
+  if (p0 < c.sinks) {
+    t.s0 = p0 >> 5;
+    t.ns = ((min(n, c.sinks) - 1) >> 5) - t.s0 + 1;
+  }
+  if (n > c.sinks) {
+    t.u0 = (max(p0, c.sinks) - c.sinks) >> 5;
+    t.nr = ((n - 1 - c.sinks) >> 5) - t.u0 + 1;
+  }
+  return t;
+}
+
+// ------------------------------------------------------------------ write ---
+struct AppendArgs {
+  Cache c;
+  const bf16 *k, *v;
+  long ldk, k_bs, ldv, v_bs;
+  const int *counts, *at;
+  int rows;
+};
+
+// Scale byte of a block whose largest magnitude has the bf16 bits `top`.
+template <int BITS> __device__ __forceinline__ int scale_byte(unsigned top) {
+  if (top >= 0x7f80) return 255;
+  top = min(top, 0x7f40u);
+  // top = 2^(e-127) (1 + m/128): the largest element is 1.5 2^2 (1.75 2^8)
+  const int e = (int)(top >> 7), m = (int)(top & 127);
+  const int s = BITS == 4 ? e - 2 + (m > 0x40) : e - 8 + (m > 0x60);
+  return min(max(s, 17), 253);
+}
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+// Codes of 8 values (element i at 4 i or 8 i bits); byte = their scale byte.
+template <int BITS> __device__ __forceinline__ u32x2 encode8(u32x4 x, int byte) {
+  u32x2 r = {0u, 0u};
+  if (byte == 255) return r;
+  const float sc = __uint_as_float((unsigned)byte << 23);
+  bf16x2 p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned w = x[i];
+    if (byte == 253 || (BITS == 8 && byte >= 246)) {      // clamp to +-1.5 2^127
+      unsigned a = w & 0x7fff, b = (w >> 16) & 0x7fff;
+      a = min(a, 0x7f40u) | (w & 0x8000u);
+      b = min(b, 0x7f40u) | ((w >> 16) & 0x8000u);
+      w = a | (b << 16);
+    }
+    p[i] = __builtin_bit_cast(bf16x2, w);
+  }
+  if constexpr (BITS == 4) {
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[0], sc, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[1], sc, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[2], sc, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, p[3], sc, 3);
+    r[0] = w;
+  } else {
+    s16x2 a = {0, 0}, b = {0, 0};
+    a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, p[0], sc, false);
+    a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, p[1], sc, true);
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, p[2], sc, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, p[3], sc, true);
+    r[0] = __builtin_bit_cast(unsigned, a);
+    r[1] = __builtin_bit_cast(unsigned, b);
+  }
+  return r;
+}
+
+// largest magnitude (bf16 bits) of 8 values, then of the 4 lanes of the block
+__device__ __forceinline__ unsigned block_top(u32x4 x) {
+  unsigned t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t = max(t, max(x[i] & 0x7fff, (x[i] >> 16) & 0x7fff));
+  t = max(t, (unsigned)__shfl_xor((int)t, 1));
+  return max(t, (unsigned)__shfl_xor((int)t, 2));
+}
+
+// One wave builds one record in LDS and stores it whole.  Lane l takes rows
+// 8 i + l / 8, i = 0..3, and the 8 values of chunk l % 8: their codes are one
+// dword (two) of the K operand; the V operand has tokens side by side, so its
+// codes are scattered as bytes, those of a token pair put together by the pair
+// of lanes l, l ^ 8 at 4 bits.  A record that keeps older tokens is read first.
+//
+// One workgroup per sequence where `whole` (its waves cover every record and
+// head, and it then stores the new state); else the records are spread over
+// blockIdx.x and advance_kernel stores the state.
+template <int BITS>
+__global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
+  constexpr int PART = kPart<BITS>, REC = kRec<BITS>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int b = blockIdx.y;
+  const int n_old = c.state[2 * b], lo_old = c.state[2 * b + 1];
+  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
+  const Span sp = write_span(c, n_old, lo_old, a.at ? a.at[b] : n_old, count);
+  Tiles t = tiles_of(c, sp.p0, sp.lo == kLost ? sp.p0 : sp.p0 + count);
+  {  // of a long write only the tiles that stay
+    const int skip = max(0, sp.lo == kLost ? 0 : sp.lo - t.u0);
+    if (t.nr > 0) { t.u0 += skip; t.nr -= skip; }
+  }
+  uint8_t* rec = lds + wave * REC;
+  const int units = (t.ns + t.nr) * c.heads;
+  for (int base = blockIdx.x * waves; base < units; base += gridDim.x * waves) {
+    const int unit = base + wave;
+    const bool on = unit < units;
+    const int ti = on ? unit / c.heads : 0, h = on ? unit - ti * c.heads : 0;
+    const bool sink = ti < t.ns;
+    const int u = sink ? t.s0 + ti : t.u0 + ti - t.ns;
+    const int pos0 = sink ? u * TOK : c.sinks + u * TOK;
+    const int pend = sink ? min(c.sinks, sp.n) : sp.n;
+    uint8_t* out = c.data + record(c, b, h, sink ? u : c.sink_tiles + u % c.ring_tiles) * REC;
+    u32x4 xk[4], xv[4];
+    bool in[4];
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = pos0 + 8 * i + (lane >> 3);
+        in[i] = p >= sp.p0 && p < pend;
+        const long r = in[i] ? p - sp.p0 : 0;
+        const int col = h * D + (lane & 7) * 8;
+        xk[i] = in[i] ? *(const u32x4*)(a.k + b * a.k_bs + r * a.ldk + col) : u32x4{0, 0, 0, 0};
+        xv[i] = in[i] ? *(const u32x4*)(a.v + b * a.v_bs + r * a.ldv + col) : u32x4{0, 0, 0, 0};
+      }
+      const bool keep = pos0 < sp.p0;
+      for (int i = lane; i < REC / 16; i += 64)
+        ((u32x4*)rec)[i] = keep ? ((const u32x4*)out)[i] : u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = 8 * i + (lane >> 3), ch = lane & 7, half = s >> 4, s16 = s & 15;
+        const int kb = scale_byte<BITS>(block_top(xk[i])), vb = scale_byte<BITS>(block_top(xv[i]));
+        const u32x2 kc = encode8<BITS>(xk[i], kb), vc = encode8<BITS>(xv[i], vb);
+        const int ks = ch >> 2, kl = (ch & 3) * 16 + s16;
+        const int g = s16 >> 2, j = half * 4 + (s & 3);
+        if constexpr (BITS == 4) {
+          if (in[i]) *(unsigned*)(rec + kl * 16 + (half * 2 + ks) * 4) = kc[0];
+          // the pair of tokens (s & ~1, s | 1) shares a byte: the even lane
+          // stores those of d = 8 ch + 0..3, the odd one of 8 ch + 4..7
+          const unsigned oc = __shfl_xor(vc[0], 8);
+          const bool oin = __shfl_xor((int)in[i], 8);
+          const bool odd = s & 1;
+          const unsigned lo4 = odd ? oc : vc[0], hi4 = odd ? vc[0] : oc;
+          const bool lin = odd ? oin : in[i], hin = odd ? in[i] : oin;
+          const unsigned mask = (lin ? 0x0fu : 0u) | (hin ? 0xf0u : 0u);
+          if (mask) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d8 = (odd ? 4 : 0) + e, d = ch * 8 + d8;
+              uint8_t* p = rec + PART + (g * 16 + (d & 15)) * 16 + (d >> 4) * 4 + (j >> 1);
+              const unsigned w = ((lo4 >> (4 * d8)) & 15u) | (((hi4 >> (4 * d8)) & 15u) << 4);
+              *p = (uint8_t)((*p & ~mask) | (w & mask));
+            }
+          }
+        } else if (in[i]) {
+          *(u32x2*)(rec + half * 1024 + kl * 16 + ks * 8) = kc;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int d = ch * 8 + e, td = d >> 4;
+            rec[PART + (td >> 1) * 1024 + (g * 16 + (d & 15)) * 16 + (td & 1) * 8 + j] =
+                (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));
+          }
+        }
+        if (in[i] && (ch & 3) == 0) {
+          rec[2 * PART + s16 * 4 + half * 2 + ks] = (uint8_t)kb;
+          rec[2 * PART + 64 + g * 16 + ks * 8 + j] = (uint8_t)vb;
+        }
+      }
+    }
+    __syncthreads();
+    if (on)
+      for (int i = lane; i < REC / 16; i += 64) ((u32x4*)out)[i] = ((const u32x4*)rec)[i];
+    __syncthreads();
+  }
+  if (whole) {
+    __syncthreads();                    // every wave has read the old state
+    if (threadIdx.x == 0) {
+      c.state[2 * b] = sp.n;
+      c.state[2 * b + 1] = sp.lo;
+    }
+  }
+}
+
+__global__ void advance_kernel(AppendArgs a, int batch) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= batch) return;
+  const int n = a.c.state[2 * b];
+  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
+  const Span s = write_span(a.c, n, a.c.state[2 * b + 1], a.at ? a.at[b] : n, count);
+  a.c.state[2 * b] = s.n;
+  a.c.state[2 * b + 1] = s.lo;
+}
+
+__global__ void reset_kernel(int* state, int batch) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < 2 * batch) state[i] = 0;
+}
+
+// --------------------------------------------------------------- decoding ---
+// The scale operand of v_cvt_scalef32_* counts by its exponent field alone, so
+// byte i of a dword becomes a scale by one shift.
+template <int I> __device__ __forceinline__ float scale_of(unsigned w) {
+  return __uint_as_float(I == 3 ? w >> 1 : w << (23 - 8 * I));
+}
+
+template <int BITS, int PAIR>             // codes 2 PAIR, 2 PAIR + 1 of 8
+__device__ __forceinline__ unsigned decode2(u32x2 w, float sc) {
+  if constexpr (BITS == 4)
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, PAIR));
+  else
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[PAIR >> 1], sc, PAIR & 1));
+}
+
+// 8 codes of one scale
+template <int BITS> __device__ __forceinline__ bf16x8 decode8(u32x2 w, float sc) {
+  const u32x4 r = {decode2<BITS, 0>(w, sc), decode2<BITS, 1>(w, sc), decode2<BITS, 2>(w, sc),
+                   decode2<BITS, 3>(w, sc)};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// 8 codes, the scale of each a byte of s0 (codes 0..3) and s1 (4..7): a pair is
+// converted with either scale and put together from the two halves
+template <int BITS> __device__ __forceinline__ bf16x8 decode8_each(u32x2 w, unsigned s0, unsigned s1) {
+  auto mix = [](unsigned lo, unsigned hi) { return (lo & 0xffffu) | (hi & 0xffff0000u); };
+  const u32x4 r = {mix(decode2<BITS, 0>(w, scale_of<0>(s0)), decode2<BITS, 0>(w, scale_of<1>(s0))),
+                   mix(decode2<BITS, 1>(w, scale_of<2>(s0)), decode2<BITS, 1>(w, scale_of<3>(s0))),
+                   mix(decode2<BITS, 2>(w, scale_of<0>(s1)), decode2<BITS, 2>(w, scale_of<1>(s1))),
+                   mix(decode2<BITS, 3>(w, scale_of<2>(s1)), decode2<BITS, 3>(w, scale_of<3>(s1)))};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// A record in a wave's registers.
+template <int BITS> struct Rec {
+  u32x4 k[BITS / 4], v[BITS / 4];
+  unsigned ks;                          // scales of token (lane & 15): [half][ks]
+  u32x4 vs;                             // scales of the lane's 8 tokens: [d >> 5][8]
+  __device__ __forceinline__ void load(const uint8_t* p, int lane) {
+    constexpr int PART = kPart<BITS>;
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) {
+      k[i] = *(const u32x4*)(p + i * 1024 + lane * 16);
+      v[i] = *(const u32x4*)(p + PART + i * 1024 + lane * 16);
+    }
+    ks = *(const unsigned*)(p + 2 * PART + (lane & 15) * 4);
+    vs = *(const u32x4*)(p + 2 * PART + 64 + (lane >> 4) * 16);
+  }
+  __device__ __forceinline__ u32x2 kw(int half, int s) const {
+    return BITS == 4 ? u32x2{k[0][half * 2 + s], 0u}
+                     : u32x2{k[BITS == 4 ? 0 : half][s * 2], k[BITS == 4 ? 0 : half][s * 2 + 1]};
+  }
+  __device__ __forceinline__ u32x2 vw(int td) const {
+    return BITS == 4 ? u32x2{v[0][td], 0u}
+                     : u32x2{v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2], v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2 + 1]};
+  }
+  template <int HALF, int S> __device__ __forceinline__ bf16x8 kfrag() const {
+    return decode8<BITS>(kw(HALF, S), scale_of<HALF * 2 + S>(ks));
+  }
+  __device__ __forceinline__ bf16x8 vfrag(int td) const {
+    return decode8_each<BITS>(vw(td), vs[(td >> 1) * 2], vs[(td >> 1) * 2 + 1]);
+  }
+};
+
+// ------------------------------------------------------------------- read ---
+struct ReadArgs {
+  Cache c;
+  bf16 *k, *v;
+  long ldk, k_bs, ldv, v_bs;
+  const int* starts;
+  int start, rows;
+};
+
+// One wave decodes one record; K leaves as the operand's own 8 values a lane,
+// V through LDS.  Rows that the cache does not hold (behind the last token,
+// fallen out of the ring, of a lost sequence) are zeros.
+template <int BITS>
+__global__ __launch_bounds__(64) void read_kernel(ReadArgs a) {
+  constexpr int LD = D + 8;
+  __shared__ __attribute__((aligned(16))) bf16 sv[TOK * LD];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int grp = lane >> 4, col = lane & 15;
+  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
+  // (positions past kMaxPos do not exist; a start out of range reads zeros)
+  const int first = min(max(a.starts ? a.starts[b] : a.start, -kMaxPos), kMaxPos - 1);
+  const int p0 = max(first, 0), p1 = first + a.rows;
+  const Tiles t = tiles_of(c, p0, p1);
+  bf16* ko = a.k + b * a.k_bs + h * D;
+  bf16* vo = a.v + b * a.v_bs + h * D;
+  const bf16x8 zero = {};
+  if (blockIdx.x == 0 && first < 0)
+    for (long i = lane; i < 8L * min(a.rows, -first); i += 64) {
+      st8(ko + (i >> 3) * a.ldk + (i & 7) * 8, zero);
+      st8(vo + (i >> 3) * a.ldv + (i & 7) * 8, zero);
+    }
+  for (int ti = blockIdx.x; ti < t.ns + t.nr; ti += gridDim.x) {
+    const bool sink = ti < t.ns;
+    const int u = sink ? t.s0 + ti : t.u0 + ti - t.ns;
+    const int pos0 = sink ? u * TOK : c.sinks + u * TOK;
+    const int pend = min(p1, sink ? c.sinks : p1);         // rows of this record to write
+    const bool held = lo != kLost && (sink || u >= lo) && pos0 < n;
+    Rec<BITS> r = {};
+    if (held) r.load(c.data + record(c, b, h, sink ? u : c.sink_tiles + u % c.ring_tiles) * kRec<BITS>, lane);
+    auto put_k = [&](int half, int s, bf16x8 x) {
+      const int p = pos0 + half * 16 + col;
+      if (p >= p0 && p < pend)
+        st8(ko + (long)(p - first) * a.ldk + s * 32 + grp * 8, held && p < n ? x : zero);
+    };
+    put_k(0, 0, r.template kfrag<0, 0>());
+    put_k(0, 1, r.template kfrag<0, 1>());
+    put_k(1, 0, r.template kfrag<1, 0>());
+    put_k(1, 1, r.template kfrag<1, 1>());
+#pragma unroll
+    for (int td = 0; td < 4; ++td) {
+      const bf16x8 x = r.vfrag(td);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sv[((j >> 2) * 16 + 4 * grp + (j & 3)) * LD + td * 16 + col] = x[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = 8 * i + (lane >> 3), p = pos0 + s;
+      if (p >= p0 && p < pend)
+        st8(vo + (long)(p - first) * a.ldv + (lane & 7) * 8,
+            held && p < n ? *(const bf16x8*)(sv + s * LD + (lane & 7) * 8) : zero);
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------- attention ---
+struct AttendArgs {
+  Cache c;
+  const bf16* q;
+  long ldq, q_bs;
+  bf16* o;
+  long ldo, o_bs;
+  const int* counts;
+  int rows, group, hq, window;
+  float scale_log2;
+  int splits;
+  float* part;                          // [batch * heads][columns][splits][D + 2]
+};
+
+// Columns: column j of a KV head is query row j / group of query head
+// j % group of the head's group, so all the query heads that share a KV head
+// share each record that a wave decodes.  A wave holds QT tiles of 16 columns;
+// KW of the workgroup's 4 waves take turns at the records of the same columns
+// and are joined through LDS, the others hold further columns.  The records of
+// a call are split over blockIdx.y too when there are few columns; the parts
+// (running maximum, sum and unscaled output) are then joined by join_kernel.
+//
+// S^T[token, column] = K . Q^T and O^T[d, column] = V^T . P^T, so a lane owns
+// one column (lane & 15); the accumulators of S^T are the operand P^T as they
+// stand.  The maximum moves only when a score passes it by 2^8 (exp2 units).
+// The sum of the rounded probabilities is an MFMA with a row of ones.
+template <int BITS, int QT, int KW>
+__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
+  constexpr int NQ = 4 / KW;                       // column groups of a workgroup
+  __shared__ float s_part[KW > 1 ? NQ * (KW - 1) * QT * 16 * (D + 2) : 1];
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int grp = lane >> 4, col = lane & 15;
+  const int b = blockIdx.z / c.heads, h = blockIdx.z - b * c.heads;
+  const int kw = wave % KW, cg = wave / KW;
+  const int ncol = a.rows * a.group;
+  const int col0 = (blockIdx.x * NQ + cg) * QT * 16;
+  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
+  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
+  const int first = n - count;                     // position of query row 0
+  // the whole call needs positions from `need`; NaN when some are gone
+  const int need = max(c.sinks, a.window ? first - a.window + 1 : 0);
+  const bool lost = lo == kLost || first < 0 || (n > c.sinks && (need - c.sinks) >> 5 < lo && need < n);
+
+  int qpos[QT];                                    // of this lane's column; -1: none
+  const bf16* qrow[QT];
+  bf16x8 qf[QT][2];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int j = min(col0 + t * 16 + col, ncol - 1);
+    const int r = j / a.group, hh = h * a.group + j - r * a.group;
+    qpos[t] = r < count && col0 + t * 16 + col < ncol ? first + r : -1;
+    qrow[t] = a.q + b * a.q_bs + r * a.ldq + hh * D;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) qf[t][s] = ld8(qrow[t] + s * 32 + grp * 8);
+  }
+  // positions of the wave's first and last column (ascending by column)
+  const int r0 = col0 / a.group, r1 = min(min(col0 + QT * 16, ncol) - 1, ncol - 1) / a.group;
+  const int qlo = first + min(r0, count - 1), qhi = first + min(r1, count - 1);
+  const bool any = r0 < count && col0 < ncol && !lost;
+
+  f32x4 o[QT][5];
+  float m_run[QT], m_thr[QT], m_off[QT];
+  const float cs = a.scale_log2;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m_run[t] = -INFINITY;
+    m_thr[t] = -INFINITY;
+    m_off[t] = 0.f;
+  }
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.0f);
+
+  if (any) {
+    const int wlo = a.window ? max(0, qlo - a.window + 1) : 0;
+    // records: the sinks that some column sees, then the ring from `wlo`
+    const int ns = (min(c.sinks, qhi + 1) + TOK - 1) / TOK;
+    const int u0 = max(wlo - c.sinks, 0) >> 5;
+    const int nr = qhi >= c.sinks ? max(((qhi - c.sinks) >> 5) - u0 + 1, 0) : 0;
+    const int total = ns + nr;
+    const int per = (total + a.splits - 1) / a.splits;
+    const int t0 = blockIdx.y * per, t1 = min(total, t0 + per);
+    const uint8_t* base = c.data + record(c, b, h, 0) * kRec<BITS>;
+    auto addr = [&](int ti) {
+      const int u = ti < ns ? ti : c.sink_tiles + (u0 + ti - ns) % c.ring_tiles;
+      return base + (long)u * kRec<BITS>;
+    };
+    Rec<BITS> r;
+    if (t0 + kw < t1) r.load(addr(t0 + kw), lane);
+    for (int ti = t0 + kw; ti < t1; ti += KW) {
+      Rec<BITS> nx;
+      nx.load(addr(min(ti + KW, t1 - 1)), lane);
+      const bool sink = ti < ns;
+      const int pos0 = sink ? ti * TOK : c.sinks + (u0 + ti - ns) * TOK;
+      const int plim = sink ? c.sinks : kMaxPos;
+      // all 32 positions are visible to every column of the wave
+      const bool full = pos0 + TOK - 1 <= qlo && pos0 + TOK <= plim &&
+                        (!a.window || pos0 > qhi - a.window || pos0 + TOK <= c.sinks);
+      const bf16x8 k00 = r.template kfrag<0, 0>(), k01 = r.template kfrag<0, 1>();
+      const bf16x8 k10 = r.template kfrag<1, 0>(), k11 = r.template kfrag<1, 1>();
+      f32x4 sc[QT][2];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k00, qf[t][0], x, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k10, qf[t][0], y, 0, 0, 0);
+        sc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k01, qf[t][1], x, 0, 0, 0);
+        sc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k11, qf[t][1], y, 0, 0, 0);
+      }
+      auto sees = [&](int t, int half, int i) {
+        const int p = pos0 + half * 16 + grp * 4 + i;
+        return p <= qpos[t] && p < plim && (!a.window || p > qpos[t] - a.window || p < c.sinks);
+      };
+      bool nanfix = false;
+      u32x4 vs = r.vs;
+      if (!full) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            sc[t][i >> 2][i & 3] = sees(t, i >> 2, i & 3) ? sc[t][i >> 2][i & 3] : -INFINITY;
+        // a NaN block of a token that some column does not see must not reach
+        // that column through 0 * NaN: look for scale bytes 0xff
+        unsigned bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= (~vs[i] - 0x01010101u) & vs[i] & 0x80808080u;
+        nanfix = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+        if (nanfix)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // (bytes never exceed 253 otherwise: 0xff is the only one with
+            // its lowest two bits and all others set)
+            unsigned w = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned x = (vs[i] >> (8 * e)) & 255u;
+              w |= (x == 255u ? 127u : x) << (8 * e);
+            }
+            r.vs[i] = w;
+          }
+      }
+      bf16x8 pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float mx = sc[t][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = smax(mx, sc[t][i >> 2][i & 3]);
+        mx = max_xor32(max_xor16(mx));
+        const bool grow = mx * cs > m_thr[t];
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+          const float m_new = smax(m_run[t], mx);
+          const float alpha = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m_new) * cs);
+#pragma unroll
+          for (int i = 0; i < 5; ++i) o[t][i] *= alpha;
+          m_run[t] = m_new;
+          m_thr[t] = m_new * cs + 8.f;
+          m_off[t] = m_new == -INFINITY ? 0.f : -m_new * cs;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          pf[t][i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t])));
+        o[t][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], o[t][4], 0, 0, 0);
+      }
+#pragma unroll
+      for (int td = 0; td < 4; ++td) {
+        const bf16x8 vf = r.vfrag(td);
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+          o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[t][td], 0, 0, 0);
+      }
+      if (nanfix) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+            bf16x8 pn;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const bool isnan = ((vs[blk * 2 + (j >> 2)] >> (8 * (j & 3))) & 255u) == 255u;
+              pn[j] = f2bf(isnan && sees(t, j >> 2, j & 3) ? __builtin_nanf("") : 0.f);
+            }
+#pragma unroll
+            for (int td = blk * 2; td < blk * 2 + 2; ++td)
+              o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pn, o[t][td], 0, 0, 0);
+          }
+      }
+      r = nx;
+    }
+  }
+
+  // join the KW waves of the same columns
+  if constexpr (KW > 1) {
+    if (kw > 0) {
+      float* sp = s_part + ((cg * (KW - 1) + kw - 1) * QT) * 16 * (D + 2);
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float* row = sp + (t * 16 + col) * (D + 2);
+#pragma unroll
+        for (int td = 0; td < 4; ++td)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) row[2 + td * 16 + grp * 4 + i] = o[t][td][i];
+        if (grp == 0) { row[0] = m_run[t]; row[1] = o[t][4][0]; }
+      }
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float m = m_run[t];
+      for (int w = 0; w < KW - 1; ++w)
+        m = smax(m, s_part[((cg * (KW - 1) + w) * QT + t) * 16 * (D + 2) + col * (D + 2)]);
+      const float al = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m) * cs);
+#pragma unroll
+      for (int i = 0; i < 5; ++i) o[t][i] *= al;
+      for (int w = 0; w < KW - 1; ++w) {
+        const float* row = s_part + ((cg * (KW - 1) + w) * QT + t) * 16 * (D + 2) + col * (D + 2);
+        const float aw = row[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((row[0] - m) * cs);
+#pragma unroll
+        for (int td = 0; td < 4; ++td)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][td][i] += aw * row[2 + td * 16 + grp * 4 + i];
+        o[t][4][0] += aw * row[1];
+      }
+      m_run[t] = m;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int j = col0 + t * 16 + col;
+    if (j >= ncol) continue;
+    if (a.splits > 1) {
+      float* row = a.part + (((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y) * (D + 2);
+#pragma unroll
+      for (int td = 0; td < 4; ++td)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row[2 + td * 16 + grp * 4 + i] = o[t][td][i];
+      if (grp == 0) { row[0] = m_run[t]; row[1] = o[t][4][0]; }
+      continue;
+    }
+    const int r = j / a.group, hh = h * a.group + j - r * a.group;
+    const float l = o[t][4][0];
+    float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a NaN sum stays one)
+    if (r >= count) inv = 0.f;
+    bf16* out = a.o + b * a.o_bs + r * a.ldo + hh * D;
+#pragma unroll
+    for (int td = 0; td < 4; ++td) {
+      bf16x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[i] = f2bf(r >= count ? 0.f : lost ? __builtin_nanf("") : o[t][td][i] * inv);
+      *reinterpret_cast<bf16x4*>(out + td * 16 + grp * 4) = y;
+    }
+  }
+}
+
+// One wave per column: joins the parts of the splits.
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int ncol = a.rows * a.group;
+  const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (j >= ncol) return;
+  const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
+  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
+  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
+  const int first = n - count;
+  const int need = max(c.sinks, a.window ? first - a.window + 1 : 0);
+  const bool lost = lo == kLost || first < 0 || (n > c.sinks && (need - c.sinks) >> 5 < lo && need < n);
+  const int r = j / a.group, hh = h * a.group + j - r * a.group;
+  const float* row = a.part + ((long)blockIdx.y * ncol + j) * a.splits * (D + 2);
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = smax(m, row[s * (D + 2)]);
+  float l = 0.f, o = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = row + s * (D + 2);
+    const float w = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((p[0] - m) * a.scale_log2);
+    l += w * p[1];
+    o += w * p[2 + lane];
+  }
+  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  a.o[b * a.o_bs + r * a.ldo + hh * D + lane] =
+      f2bf(r >= count ? 0.f : lost ? __builtin_nanf("") : o * inv);
+}
+
+bool cache_ok(const svla_kv_cache* c) {
+  return c && c->data && c->state && svla_aligned16(c->data) && c->batch > 0 && c->n_kv_heads > 0 &&
+         c->head_dim == D && (c->format == SVLA_KV_MXFP4 || c->format == SVLA_KV_MXFP8) &&
+         c->sinks >= 0 && c->sinks <= kMaxPos / 2 && c->ring >= TOK && c->ring % TOK == 0 &&
+         c->ring <= kMaxPos && c->batch <= 65535 / c->n_kv_heads;
+}
+
+Cache device_cache(const svla_kv_cache* c) {
+  Cache d;
+  d.data = static_cast<uint8_t*>(c->data);
+  d.state = c->state;
+  d.heads = c->n_kv_heads;
+  d.sinks = c->sinks;
+  d.sink_tiles = (c->sinks + TOK - 1) / TOK;
+  d.ring_tiles = c->ring / TOK;
+  return d;
+}
+
+bool rows_ok(const void* p, int ld, long bs, int heads) {
+  return p && svla_aligned16(p) && ld % 8 == 0 && bs % 8 == 0 && ld >= heads * D;
+}
+
+// splits of a call whose columns fill `wgs` workgroups of `kw` key waves over
+// at most `tiles` records
+int pick_splits(long wgs, int kw, long tiles) {
+  const long per_wave = 8;                       // records that a wave should get at least
+  long s = (2 * 256 + wgs - 1) / wgs;
+  s = min(s, (tiles + kw * per_wave - 1) / (kw * per_wave));
+  return (int)max(1L, min(s, 128L));
+}
+
+struct Plan {
+  int qt, kw, splits;
+  dim3 grid;
+};
+
+Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
+  Plan p;
+  const long ncol = (long)rows * (hq / c->n_kv_heads);
+  const long bh = (long)c->batch * c->n_kv_heads;
+  p.qt = 1;
+  p.kw = ncol <= 16 ? 4 : 1;
+  const int nq = 4 / p.kw;
+  const long cols = 16L * p.qt * nq;
+  const long x = (ncol + cols - 1) / cols;
+  const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
+  const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
+  p.splits = p.kw == 4 ? pick_splits(x * bh, p.kw, tiles) : 1;
+  p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+long svla_kv_cache_bytes(int batch, int n_kv_heads, int head_dim, int format, int sinks, int ring) {
+  svla_kv_cache c = {(void*)16, (int*)16, batch, n_kv_heads, head_dim, format, sinks, ring};
+  if (!cache_ok(&c)) return 0;
+  const long rec = format == SVLA_KV_MXFP4 ? kRec<4> : kRec<8>;
+  return (long)batch * n_kv_heads * ((sinks + TOK - 1) / TOK + ring / TOK) * rec;
+}
+
+int svla_kv_reset(const svla_kv_cache* c, svla_stream_t stream) {
+  if (!cache_ok(c)) return SVLA_EINVAL;
+  hipLaunchKernelGGL(reset_kernel, dim3((2 * c->batch + 255) / 256), dim3(256), 0,
+                     (hipStream_t)stream, c->state, c->batch);
+  SVLA_CHECK_LAUNCH();
+  return SVLA_OK;
+}
+
+int svla_kv_append_bf16(const svla_kv_cache* c, const void* k, int ldk, long k_bs, const void* v,
+                        int ldv, long v_bs, int rows, const int* counts, const int* at,
+                        svla_stream_t stream) {
+  if (!cache_ok(c) || rows < 0 || rows > kMaxPos) return SVLA_EINVAL;
+  if (rows == 0 && !at) return SVLA_OK;
+  if (rows > 0 && (!rows_ok(k, ldk, k_bs, c->n_kv_heads) || !rows_ok(v, ldv, v_bs, c->n_kv_heads)))
+    return SVLA_EINVAL;
+  AppendArgs a;
+  a.c = device_cache(c);
+  a.k = static_cast<const bf16*>(k); a.ldk = ldk; a.k_bs = k_bs;
+  a.v = static_cast<const bf16*>(v); a.ldv = ldv; a.v_bs = v_bs;
+  a.counts = counts;
+  a.at = at;
+  a.rows = rows;
+  hipStream_t s = (hipStream_t)stream;
+  // records that `rows` consecutive positions touch, at most
+  long tiles = rows ? (rows + TOK - 2) / TOK + 1 + (c->sinks && rows > 1) : 1;
+  tiles = min(tiles, (long)a.c.ring_tiles + a.c.sink_tiles);
+  const long units = tiles * c->n_kv_heads;
+  const size_t rec = c->format == SVLA_KV_MXFP4 ? kRec<4> : kRec<8>;
+  const bool whole = units <= 12;          // 12 records of 8 bits: 51 KB of LDS
+  const int waves = whole ? (int)units : 4;
+  const dim3 grid(whole ? 1 : (unsigned)min((units + 3) / 4, 1L << 20), c->batch);
+  if (c->format == SVLA_KV_MXFP4)
+    hipLaunchKernelGGL(append_kernel<4>, grid, dim3(64 * waves), waves * rec, s, a, (int)whole);
+  else
+    hipLaunchKernelGGL(append_kernel<8>, grid, dim3(64 * waves), waves * rec, s, a, (int)whole);
+  SVLA_CHECK_LAUNCH();
+  if (!whole) {
+    hipLaunchKernelGGL(advance_kernel, dim3((c->batch + 255) / 256), dim3(256), 0, s, a, c->batch);
+    SVLA_CHECK_LAUNCH();
+  }
+  return SVLA_OK;
+}
+
+int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void* v, int ldv,
+                      long v_bs, int start, const int* starts, int rows, svla_stream_t stream) {
+  if (!cache_ok(c) || rows < 0 || rows > kMaxPos || (!starts && (start < 0 || start > kMaxPos)))
+    return SVLA_EINVAL;
+  if (rows == 0) return SVLA_OK;
+  if (!rows_ok(k, ldk, k_bs, c->n_kv_heads) || !rows_ok(v, ldv, v_bs, c->n_kv_heads))
+    return SVLA_EINVAL;
+  ReadArgs a;
+  a.c = device_cache(c);
+  a.k = static_cast<bf16*>(k); a.ldk = ldk; a.k_bs = k_bs;
+  a.v = static_cast<bf16*>(v); a.ldv = ldv; a.v_bs = v_bs;
+  a.starts = starts;
+  a.start = start;
+  a.rows = rows;
+  const long tiles = (rows + TOK - 2) / TOK + 1 + (c->sinks > 0);
+  const dim3 grid((unsigned)min(tiles, 1L << 20), c->n_kv_heads, c->batch);
+  if (c->format == SVLA_KV_MXFP4)
+    hipLaunchKernelGGL(read_kernel<4>, grid, dim3(64), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(read_kernel<8>, grid, dim3(64), 0, (hipStream_t)stream, a);
+  SVLA_CHECK_LAUNCH();
+  return SVLA_OK;
+}
+
+long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window) {
+  if (!cache_ok(c) || rows <= 0 || hq <= 0 || hq % c->n_kv_heads || window < 0) return 0;
+  const Plan p = plan_attend(c, rows, hq, window);
+  return p.splits > 1 ? (long)c->batch * hq * rows * p.splits * (D + 2) * 4 : 0;
+}
+
+int svla_kv_attention_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o,
+                           int ldo, long o_bs, int rows, const int* counts, int hq, float scale,
+                           int window, void* scratch, long scratch_bytes, svla_stream_t stream) {
+  if (!cache_ok(c) || rows < 0 || hq <= 0 || hq % c->n_kv_heads || window < 0 ||
+      !(scale > 0.f) || !(scale < 1e30f))
+    return SVLA_EINVAL;
+  if (rows == 0) return SVLA_OK;
+  if ((long)rows * hq > (1L << 24)) return SVLA_EINVAL;
+  if (!rows_ok(q, ldq, q_bs, hq) || !o || ((uintptr_t)o & 7) || ldo % 4 || o_bs % 4 || ldo < hq * D)
+    return SVLA_EINVAL;
+  const Plan p = plan_attend(c, rows, hq, window);
+  if (svla_kv_attention_scratch(c, rows, hq, window) > scratch_bytes ||
+      (p.splits > 1 && (!scratch || ((uintptr_t)scratch & 3))))
+    return SVLA_EINVAL;
+  AttendArgs a;
+  a.c = device_cache(c);
+  a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.q_bs = q_bs;
+  a.o = static_cast<bf16*>(o); a.ldo = ldo; a.o_bs = o_bs;
+  a.counts = counts;
+  a.rows = rows;
+  a.hq = hq;
+  a.group = hq / c->n_kv_heads;
+  a.window = min(window, kMaxPos);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = p.splits;
+  a.part = static_cast<float*>(scratch);
+  hipStream_t s = (hipStream_t)stream;
+  const bool f4 = c->format == SVLA_KV_MXFP4;
+  if (p.kw == 4) {
+    if (f4) hipLaunchKernelGGL((attend_kernel<4, 1, 4>), p.grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<8, 1, 4>), p.grid, dim3(256), 0, s, a);
+  } else {
+    if (f4) hipLaunchKernelGGL((attend_kernel<4, 1, 1>), p.grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<8, 1, 1>), p.grid, dim3(256), 0, s, a);
+  }
+  SVLA_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    const dim3 grid((rows * a.group + 3) / 4, p.grid.z);
+    hipLaunchKernelGGL(join_kernel, grid, dim3(256), 0, s, a);
+    SVLA_CHECK_LAUNCH();
+  }
+  return SVLA_OK;
+}
+
+}  // extern "C"

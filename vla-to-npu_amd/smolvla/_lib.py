@@ -44,6 +44,14 @@ class ExpertPlan(ctypes.Structure):
                 ("spin_limit", ctypes.c_int), ("stamps", _p)]
 
 
+class KVCacheDesc(ctypes.Structure):
+    """``svla_kv_cache`` (include/svla.h)."""
+    _fields_ = [("data", _p), ("state", _p)] + [(n, ctypes.c_int) for n in (
+        "batch", "n_kv_heads", "head_dim", "format", "sinks", "ring")]
+
+
+_kv = ctypes.POINTER(KVCacheDesc)
+
 # name -> argtypes (all return int, except RESTYPES)
 SIGNATURES = {
     "svla_version": [],
@@ -75,6 +83,8 @@ SIGNATURES = {
                             _i, _f, _i, _i, _p],
     "svla_attention_lo_bf16": [_p, _p, _i, _l, _p, _p, _i, _l, _p, _i, _l, _p, _i, _l, _i, _i, _i,
                                _i, _i, _i, _f, _i, _i, _p],
+    "svla_attention_window_bf16": [_p, _i, _l, _p, _i, _l, _p, _i, _l, _p, _i, _l, _i, _i, _i, _i,
+                                   _i, _i, _f, _i, _p, _i, _i, _p],
     "svla_masked_softmax_bf16": [_p, _i, _p, _i, _i, _p],
     "svla_softmax": [_p, _p, _i, _i, _i, _i, _p],
     "svla_silu_bf16": [_p, _p, _l, _p],
@@ -100,10 +110,18 @@ SIGNATURES = {
     "svla_expert_run": [ctypes.POINTER(ExpertPlan), _p],
     "svla_expert_status": [ctypes.POINTER(ExpertPlan), ctypes.POINTER(ctypes.c_int)],
     "svla_expert_trace_offset": [ctypes.POINTER(ExpertDesc), _i, _i],
+    "svla_kv_cache_bytes": [_i, _i, _i, _i, _i, _i],
+    "svla_kv_reset": [_kv, _p],
+    "svla_kv_append_bf16": [_kv, _p, _i, _l, _p, _i, _l, _i, _p, _p, _p],
+    "svla_kv_read_bf16": [_kv, _p, _i, _l, _p, _i, _l, _i, _p, _i, _p],
+    "svla_kv_attention_scratch": [_kv, _i, _i, _i],
+    "svla_kv_attention_bf16": [_kv, _p, _i, _l, _p, _i, _l, _i, _p, _i, _f, _i, _p, _l, _p],
 }
 
 RESTYPES = {"svla_expert_workspace_size": ctypes.c_long,
-            "svla_expert_trace_offset": ctypes.c_long}
+            "svla_expert_trace_offset": ctypes.c_long,
+            "svla_kv_cache_bytes": ctypes.c_long,
+            "svla_kv_attention_scratch": ctypes.c_long}
 
 _LIB = None
 

@@ -364,13 +364,50 @@ def action_out_euler(a, w, x_f32, dt, x_bf16=None, norm=None):
 
 
 # ------------------------------------------------------------- attention ---
+def _attention_window(q, k, v, out, hq, hkv, scale, window, sinks, lens, q_pos):
+    B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
+    if window is None:
+        raise ValueError('attention: mask="window" needs window')
+    if not q.is_cuda:
+        raise ValueError("smolvla ops take GPU tensors (no CPU fallback)")
+    for t, rows, heads in ((q, Sq, hq), (k, Sk, hkv), (v, Sk, hkv), (out, Sq, hq)):
+        if (t.dtype != BF16 or t.device != q.device or t.shape[:2] != (B, rows)
+                or t.shape[2] < heads * 64):
+            raise ValueError(f"attention: bf16 [{B}, {rows}, {heads * 64}] on {q.device} expected, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,)
+                             or not lens.is_contiguous() or lens.device != q.device):
+        raise ValueError(f"attention: lens must be contiguous int32 [{B}] on {q.device}")
+
+    # (a stride that no index uses need not be a valid one)
+    def ld(t):
+        return t.stride(1) if t.shape[1] > 1 else (t.shape[2] + 7) // 8 * 8
+
+    def bs(t):
+        return t.stride(0) if B > 1 else 0
+
+    with torch.cuda.device(q.device):
+        _lib.call("svla_attention_window_bf16", _ptr(q), ld(q), bs(q), _ptr(k), ld(k), bs(k),
+                  _ptr(v), ld(v), bs(v), _ptr(out), ld(out), bs(out), B, Sq, Sk, hq, hkv, 64,
+                  float(scale), int(q_pos), _ptr(lens), int(window), int(sinks), _stream())
+    return out
+
+
 def attention(q, k, v, out, hq, hkv, mask="causal", prefix_len=0, scale=None, q_lo=None,
-              k_lo=None):
+              k_lo=None, window=None, sinks=0, lens=None, q_pos=0):
     """``q [B, Sq, >=hq*64]``, ``k``/``v [B, Sk, >=hkv*64]`` (views into fused
     projection buffers are fine: row stride = ``stride(1)``), ``out [B, Sq, hq*64]``.
     ``q_lo`` / ``k_lo``: bf16 remainders of fp32 Q / K (views with q's / k's
     strides, from :func:`linear_rope`'s ``out_lo``): the scores are then taken
-    on Q = q + q_lo, K = k + k_lo (``svla_attention_lo_bf16``)."""
+    on Q = q + q_lo, K = k + k_lo (``svla_attention_lo_bf16``).
+
+    ``mask="window"``: query row r, at position ``q_pos + r``, sees the keys
+    (key j at position j) up to its own position that are within the last
+    ``window`` or among the first ``sinks``; of sequence b only the first
+    ``lens[b]`` keys (int32 ``[B]`` on the device) exist.  A row that sees none
+    gives zeros (``svla_attention_window_bf16``)."""
+    if mask != "window" and (window is not None or sinks or lens is not None or q_pos):
+        raise ValueError('attention: window, sinks, lens and q_pos go with mask="window"')
     B, Sq = q.shape[0], q.shape[1]
     Sk = k.shape[1]
     for t in (q, k, v, out):
@@ -380,6 +417,10 @@ def attention(q, k, v, out, hq, hkv, mask="causal", prefix_len=0, scale=None, q_
         if lo is not None and (lo.shape != hi.shape or lo.stride() != hi.stride()):
             raise ValueError("attention: a remainder needs its operand's shape and strides")
     scale = 1.0 / math.sqrt(64) if scale is None else scale
+    if mask == "window":
+        if q_lo is not None or k_lo is not None or prefix_len:
+            raise ValueError("attention: no remainders and no prefix with a window")
+        return _attention_window(q, k, v, out, hq, hkv, scale, window, sinks, lens, q_pos)
     _lib.call("svla_attention_lo_bf16",
               _ptr(q), _ptr(q_lo), q.stride(1), q.stride(0), _ptr(k), _ptr(k_lo), k.stride(1),
               k.stride(0), _ptr(v), v.stride(1), v.stride(0), _ptr(out), out.stride(1),
