@@ -19,6 +19,7 @@ struct WindowArgs {
   const int* lens;
   int sq, sk, hq, hkv, q_pos, window, sinks;
   float scale_log2;
+  int row_blocks, blocks, run;          // of a KV head, of the call, dealt at a time
 };
 
 // Elements of 8 bf16 that are infinite or NaN: bit 15 / 31 of every dword
@@ -28,19 +29,30 @@ __device__ __forceinline__ u32x4 nonfinite(u32x4 w) {
   return w;
 }
 
+// The loop: blocks of 64 keys go through registers into two LDS stages, so that
+// a block's loads have the whole of the block before them to arrive.
 template <int QT>
-__global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs p) {
+__global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs p) {
   constexpr int QW = 16 * QT, BQ = 4 * QW;
-  __shared__ __attribute__((aligned(1024))) bf16 sK0[BKEY * D], sK1[BKEY * D], sK2[BKEY * D];
-  __shared__ __attribute__((aligned(1024))) bf16 sV0[BKEY * D], sV1[BKEY * D], sV2[BKEY * D];
+  // K of two stages, then V of two: 8 KB each
+  constexpr int STAGE = BKEY * D * 2, V_AT = 2 * STAGE;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * STAGE];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int kvh = h * p.hkv / p.hq;
-  const int q0 = blockIdx.x * BQ;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Workgroup i runs on XCD i % 8.  The row blocks of all (sequence, KV head)s
+  // are dealt to the XCDs in runs of `run`, all query heads of a block in a
+  // row, so that what one XCD works on at a time shares keys in its L2.
+  const int group = p.hq / p.hkv;
+  const unsigned slot = blockIdx.x >> 3;
+  const unsigned in_run = slot % (p.run * group);
+  const unsigned blk_id = (slot / (p.run * group) * 8 + (blockIdx.x & 7)) * p.run + in_run / group;
+  if (blk_id >= (unsigned)p.blocks) return;
+  const int bk = blk_id / p.row_blocks;            // (sequence, KV head)
+  const int b = bk / p.hkv, kvh = bk - b * p.hkv;
+  const int h = kvh * group + in_run % group;
+  const int q0 = (blk_id - bk * p.row_blocks) * BQ;
   const int grp = lane >> 4, col = lane & 15;
   const int qw = q0 + wave * QW;
-  const bf16* qb = p.q + b * p.q_bs + h * D;
   const bf16* kb = p.k + b * p.k_bs + kvh * D;
   const bf16* vb = p.v + b * p.v_bs + kvh * D;
   const int len = p.lens ? min(max(p.lens[b], 0), p.sk) : p.sk;
@@ -52,76 +64,115 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs p) {
   const int nb = sink_blocks + max((pend + BKEY - 1) / BKEY - from, 0);
   auto key0 = [&](int blk) { return (blk < sink_blocks ? blk : from + blk - sink_blocks) * BKEY; };
 
-  long koff[2], voff[2];
+  // rows tid / 8 and 32 + tid / 8 of a block, 16 bytes each (rows past the last
+  // key repeat it: never seen)
+  u32x4 rk[2], rv[2];
+  const int srow = tid >> 3, schunk = (tid & 7) * 8;
+  const unsigned kstep = 2u * p.ldk, vstep = 2u * p.ldv;           // bytes of a row
+  const unsigned kvo = srow * kstep + schunk * 2, vvo = srow * vstep + schunk * 2;
+  const char *gk, *gv;                 // block `next`
+  int next, next_key;
+  auto start = [&]() {
+    next = 0;
+    next_key = key0(0);
+    gk = (const char*)(kb + (long)next_key * p.ldk);
+    gv = (const char*)(vb + (long)next_key * p.ldv);
+  };
+  auto load = [&]() __attribute__((always_inline)) {
+    if (next_key + BKEY <= p.sk) {
+      rk[0] = *(const u32x4*)(gk + kvo);
+      rk[1] = *(const u32x4*)(gk + 32 * kstep + kvo);
+      rv[0] = *(const u32x4*)(gv + vvo);
+      rv[1] = *(const u32x4*)(gv + 32 * vstep + vvo);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int key = (wave * 2 + j) * 8 + (lane >> 3);
-    const int c = (lane & 7) ^ (key & 7);
-    koff[j] = (long)key * p.ldk + c * 8;
-    voff[j] = (long)key * p.ldv + c * 8;
-  }
-  auto issue = [&](auto SI, int blk) {
-    constexpr int S = decltype(SI)::value;
-    bf16* sk = S == 0 ? sK0 : S == 1 ? sK1 : sK2;
-    bf16* sv = S == 0 ? sV0 : S == 1 ? sV1 : sV2;
-    const int k0 = key0(min(blk, nb - 1));
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int key = (wave * 2 + j) * 8 + (lane >> 3);
-      const int rows_left = p.sk - 1 - k0;
-      const long adj = key > rows_left ? (long)(rows_left - key) : 0;
-      const bf16* gk = kb + (long)k0 * p.ldk + koff[j] + adj * p.ldk;
-      const bf16* gv = vb + (long)k0 * p.ldv + voff[j] + adj * p.ldv;
-      __builtin_amdgcn_global_load_lds((void*)gk, (lds_ptr_t)(sk + (wave * 2 + j) * 512), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((void*)gv, (lds_ptr_t)(sv + (wave * 2 + j) * 512), 16, 0, 0);
+      for (int i = 0; i < 2; ++i) {
+        const unsigned r = min(srow + 32 * i, p.sk - 1 - next_key);
+        rk[i] = *(const u32x4*)(gk + (r * kstep + schunk * 2));
+        rv[i] = *(const u32x4*)(gv + (r * vstep + schunk * 2));
+      }
     }
+    // (past the last block: that one again, never used)
+    if (++next < nb) {
+      const int step = next == sink_blocks ? (from - sink_blocks + 1) * BKEY : BKEY;
+      next_key += step;
+      gk += (long)step * kstep;
+      gv += (long)step * vstep;
+    } else {
+      next = nb - 1;
+    }
+  };
+  int sofs = 2 * kv_off(srow, schunk);
+  auto store = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *(u32x4*)(lds + sofs + 32 * i * D * 2) = rk[i];
+      *(u32x4*)(lds + sofs + V_AT + 32 * i * D * 2) = rv[i];
+    }
+    sofs ^= STAGE;
   };
 
   bf16x8 qf[QT][2];
-  int qpos[QT];
+  int last[QT], before[QT];       // keys of this lane's row: (before, last] and sinks
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int qi = min(qw + qt * 16 + col, p.sq - 1);
-    qpos[qt] = p.q_pos + qi;
+    last[qt] = min(p.q_pos + qi, len - 1);
+    before[qt] = p.q_pos + qi - p.window;
+    const bf16* q = p.q + b * p.q_bs + (long)qi * p.ldq + h * D;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) qf[qt][ks] = ld8(qb + (long)qi * p.ldq + ks * 32 + grp * 8);
+    for (int ks = 0; ks < 2; ++ks) qf[qt][ks] = ld8(q + ks * 32 + grp * 8);
   }
   // positions of the wave's first and last row
   const int wlo = p.q_pos + min(qw, p.sq - 1), whi = p.q_pos + min(qw + QW, p.sq) - 1;
 
   f32x4 o[QT][5];
-  float m_run[QT], m_thr[QT], m_off[QT];
+  float m_run[QT], m_off[QT];
   const float c = p.scale_log2;
+  auto clear = [&]() {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
+    for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
-    for (int t = 0; t < 5; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m_run[qt] = -INFINITY;
-    m_thr[qt] = -INFINITY;
-    m_off[qt] = 0.f;
-  }
+      for (int t = 0; t < 5; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[qt] = -INFINITY;
+      m_off[qt] = 0.f;
+    }
+  };
+  clear();
   bf16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.0f);
+  int track = 0;           // follow the maximum in every block
+  bool started = false;    // every row of the wave has seen a key
 
-  auto compute = [&](auto SI, int blk) {
-    constexpr int S = decltype(SI)::value;
-    const bf16* sk = S == 0 ? sK0 : S == 1 ? sK1 : sK2;
-    const bf16* sv = S == 0 ? sV0 : S == 1 ? sV1 : sV2;
-    const int k0 = key0(blk);
-    if (qw >= p.sq || k0 > whi || (k0 + BKEY - 1 <= wlo - p.window && k0 >= p.sinks)) return;
-    const bool full = k0 + BKEY - 1 <= wlo && k0 + BKEY <= len &&
-                      (k0 > whi - p.window || k0 + BKEY <= p.sinks);
-    auto sees = [&](int qt, int key) {
-      return key <= qpos[qt] && key < len && (key > qpos[qt] - p.window || key < p.sinks);
-    };
-    f32x4 sacc[4][QT];
+  // Byte offsets of the lane's operand reads within a stage (kv_off: a key's row
+  // is 128 bytes, its 16-byte chunks are swapped by the key's low bits, which
+  // steps of 16 keys keep).
+  int kofs[2], vofs[4];
 #pragma unroll
-    for (int ts = 0; ts < 4; ++ts) {
+  for (int ks = 0; ks < 2; ++ks) kofs[ks] = 2 * kv_off(col, ks * 32 + grp * 8);
+#pragma unroll
+  for (int td = 0; td < 4; ++td) vofs[td] = 2 * kv_off(4 * grp + (col >> 2), td * 16 + 4 * (col & 3));
+
+  auto sees = [&](int qt, int key) {
+    return key <= last[qt] && (key > before[qt] || key < p.sinks);
+  };
+  f32x4 sacc[2][QT];
+  bf16x8 vf[4];
+  auto v_frag = [&](int hf, int td) __attribute__((always_inline)) {
+    const char* at = lds + vofs[td] + (V_AT + hf * 32 * D * 2);
+    const v4i16 w8[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)at),
+                         __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)(at + 16 * D * 2))};
+    return *reinterpret_cast<const bf16x8*>(w8);
+  };
+  // scores of half hf of the block, and its V
+  auto score = [&](int hf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ts = 0; ts < 2; ++ts) {
       bf16x8 kf[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
-        kf[ks] = *reinterpret_cast<const bf16x8*>(&sk[kv_off(ts * 16 + col, ks * 32 + grp * 8)]);
+        kf[ks] = *reinterpret_cast<const bf16x8*>(lds + kofs[ks] + (hf * 2 + ts) * 16 * D * 2);
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
@@ -131,138 +182,191 @@ __global__ __launch_bounds__(256, 2) void window_kernel(WindowArgs p) {
         sacc[ts][qt] = a;
       }
     }
-    bf16x8 pf[QT][2];
+#pragma unroll
+    for (int td = 0; td < 4; ++td) vf[td] = v_frag(hf, td);
+  };
+  // Masks the scores of the keys k0 .. k0 + 31: of (before, last] and the sinks
+  // the row's own are left.
+  auto mask = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      if (!full) {
+      const int at = k0 + grp * 4 - before[qt] - 1, n = max(last[qt] - before[qt], 0);
 #pragma unroll
-        for (int ts = 0; ts < 4; ++ts)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sacc[ts][qt][i] = sees(qt, k0 + ts * 16 + grp * 4 + i) ? sacc[ts][qt][i] : -INFINITY;
+      for (int i = 0; i < 8; ++i) {
+        const int key = (i >> 2) * 16 + (i & 3);
+        bool in = (unsigned)(at + key) < (unsigned)n;
+        if (k0 < p.sinks) in = sees(qt, k0 + grp * 4 + key);
+        sacc[i >> 2][qt][i & 3] = in ? sacc[i >> 2][qt][i & 3] : -INFINITY;
       }
+    }
+  };
+  // Follows the maximum, which moves only when a score passes it by 2^8 as in
+  // attention_kernel.
+  auto follow = [&]() __attribute__((always_inline)) {
+    bool seen_all = true;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
       float mx = sacc[0][qt][0];
 #pragma unroll
-      for (int ts = 0; ts < 4; ++ts)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = smax(mx, sacc[ts][qt][i]);
+      for (int i = 1; i < 8; ++i) mx = smax(mx, sacc[i >> 2][qt][i & 3]);
       mx = max_xor32(max_xor16(mx));
-      // the maximum moves only when a score passes it by 2^8 (attention_kernel)
-      const bool grow = mx * c > m_thr[qt];
+      const bool grow = mx * c > m_run[qt] * c + 8.f;
       if (__builtin_amdgcn_ballot_w64(grow)) {
         const float m_new = smax(m_run[qt], mx);
         const float alpha = m_run[qt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[qt] - m_new) * c);
 #pragma unroll
         for (int t = 0; t < 5; ++t) o[qt][t] *= alpha;
         m_run[qt] = m_new;
-        m_thr[qt] = m_new * c + 8.f;
         m_off[qt] = -((m_new == -INFINITY ? 0.f : m_new) * c);
       }
+      seen_all = seen_all && m_run[qt] != -INFINITY;
     }
+    started = __builtin_amdgcn_ballot_w64(!seen_all) == 0;
+  };
+  // Takes infinities and NaNs out of V; returns whether there were any.
+  auto take_out = [&]() __attribute__((always_inline)) {
+    unsigned some = 0;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 vf[4];
+    for (int td = 0; td < 4; ++td) {
+      u32x4 w = __builtin_bit_cast(u32x4, vf[td]);
+      const u32x4 bad = nonfinite(w);
 #pragma unroll
-      for (int td = 0; td < 4; ++td) {
-        const v4i16 lo = v_tr_read(sv, kk * 32 + 4 * grp, td * 16, col);
-        const v4i16 hi = v_tr_read(sv, kk * 32 + 16 + 4 * grp, td * 16, col);
-        const v4i16 w8[2] = {lo, hi};
-        vf[td] = *reinterpret_cast<const bf16x8*>(w8);
+      for (int i = 0; i < 4; ++i) {
+        some |= bad[i];
+        w[i] &= ~((bad[i] >> 15) * 0xffffu);
       }
-      // A row must not meet what it does not see, not even as 0 * NaN: where a
-      // block has keys that some row does not see and V holds infinities or
-      // NaNs, those are taken out of V and added to the rows that see them,
-      // found by products of indicators.
-      if (!full) {
-        u32x4 bad[4];
-        unsigned some = 0;
+      vf[td] = __builtin_bit_cast(bf16x8, w);
+    }
+    return __builtin_amdgcn_ballot_w64(some != 0) != 0;
+  };
+  auto accumulate = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int td = 0; td < 4; ++td) {
-          bad[td] = nonfinite(__builtin_bit_cast(u32x4, vf[td]));
-          some |= bad[td][0] | bad[td][1] | bad[td][2] | bad[td][3];
-        }
-        if (__builtin_amdgcn_ballot_w64(some != 0)) {
+    for (int qt = 0; qt < QT; ++qt) {
+      bf16x8 pf;
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            bf16x8 vis;
+      for (int i = 0; i < 8; ++i)
+        pf[i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i >> 2][qt][i & 3], c, m_off[qt])));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              vis[j] = f2bf(sees(qt, k0 + kk * 32 + (j >> 2) * 16 + grp * 4 + (j & 3)) ? 1.f : 0.f);
+      for (int td = 0; td < 4; ++td)
+        o[qt][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[td], pf, o[qt][td], 0, 0, 0);
+      o[qt][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf, o[qt][4], 0, 0, 0);
+    }
+  };
+  // Gives them to the rows that see them: how often each row sees +inf, -inf and
+  // NaN in each depth of the V of keys k0 .. k0 + 31, as products of indicators.
+  auto put_back = [&](int hf, int k0) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int it = 0; it < 12; ++it) {
+      const int td = it / 3, what = it % 3;
+      const bf16x8 x = td < 2 ? (td == 0 ? v_frag(hf, 0) : v_frag(hf, 1))
+                              : (td == 2 ? v_frag(hf, 2) : v_frag(hf, 3));
+      const float add = what == 0 ? INFINITY : what == 1 ? -INFINITY : __builtin_nanf("");
+      bf16x8 hit;
 #pragma unroll
-            for (int td = 0; td < 4; ++td)
-#pragma unroll
-              for (int what = 0; what < 3; ++what) {   // +inf, -inf, NaN
-                bf16x8 hit;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float x = bf2f(vf[td][j]);
-                  const bool is = what == 0 ? x == INFINITY : what == 1 ? x == -INFINITY : x != x;
-                  hit[j] = f2bf(is ? 1.f : 0.f);
-                }
-                f32x4 cnt = {0.f, 0.f, 0.f, 0.f};
-                cnt = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hit, vis, cnt, 0, 0, 0);
-                const float add = what == 0 ? INFINITY : what == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[qt][td][i] += cnt[i] > 0.f ? add : 0.f;
-              }
-          }
-#pragma unroll
-          for (int td = 0; td < 4; ++td) {
-            u32x4 w = __builtin_bit_cast(u32x4, vf[td]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] &= ((bad[td][i] & 0x8000u) ? 0u : 0xffffu) | ((bad[td][i] >> 31) ? 0u : 0xffff0000u);
-            vf[td] = __builtin_bit_cast(bf16x8, w);
-          }
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float y = bf2f(x[j]);
+        hit[j] = f2bf((what == 2 ? y != y : y == add) ? 1.f : 0.f);
       }
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
+        bf16x8 vis;
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
+        for (int j = 0; j < 8; ++j)
+          vis[j] = f2bf(sees(qt, k0 + (j >> 2) * 16 + grp * 4 + (j & 3)) ? 1.f : 0.f);
+        f32x4 cnt = {0.f, 0.f, 0.f, 0.f};
+        cnt = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hit, vis, cnt, 0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            pf[qt][kk][hh * 4 + i] =
-                f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sacc[2 * kk + hh][qt][i], c, m_off[qt])));
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int td = 0; td < 4; ++td)
-          o[qt][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[td], pf[qt][kk], o[qt][td], 0, 0, 0);
-        o[qt][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[qt][kk], o[qt][4], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) o[qt][t][i] += t == td && cnt[i] > 0.f ? add : 0.f;
       }
     }
   };
 
-  // Before each barrier: vmcnt(4), the next stage's 4 DMA instructions stay in
-  // flight, and lgkmcnt(0), this wave's reads of the stage that the DMA issued
-  // right after the barrier refills are done.
+  // lgkmcnt(0): this wave's reads of the stage that is written next, and its own
+  // writes, are done; loads into registers stay in flight
   auto sync_step = [&]() __attribute__((always_inline)) {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0x074);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
   };
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  __builtin_amdgcn_s_waitcnt(0xF70);   // Q is here before the DMA prologue
-  if (nb > 0) {                        // uniform across the workgroup
-    issue(I0{}, 0);
-    issue(I1{}, 1);
-    for (int blk = 0; blk < nb; blk += 3) {
+  // Only the first keys set the maximum: any reference gives the same quotient
+  // as long as nothing overflows.  Where something does (scores over 2^100 times
+  // the first ones, V that large, infinite or NaN: also behind the mask, as
+  // 0 * NaN), the workgroup goes over its keys once more, following the maximum,
+  // and a row then meets only what it sees, infinities and NaNs apart.
+  // The wave's blocks in the list: [see0, see1) of the windows' blocks hold keys
+  // that some row sees, [full0, full1) only keys that all do; of the sinks' the
+  // first sink_full.
+  const int shift = sink_blocks - from;
+  const int see0 = max(max(wlo - p.window + 1, 0) / BKEY + shift, sink_blocks);
+  const int see1 = qw < p.sq ? min(whi / BKEY + 1 + shift, nb) : 0;
+  const int full0 = (max(whi - p.window + 1, 0) + BKEY - 1) / BKEY + shift;
+  const int full1 = min(wlo + 1, len) / BKEY + shift;
+  const int sink_full = min(min(wlo + 1, len), p.sinks) / BKEY;
+  const int sink_see = qw < p.sq ? sink_blocks : 0;
+  for (;;) {
+    if (nb > 0) {                      // uniform across the workgroup
+      start();
+      load();
+      store();
+      load();
       sync_step();
-      issue(I2{}, blk + 2);
-      compute(I0{}, blk);
-      if (blk + 1 >= nb) break;
+    }
+    for (int blk = 0; blk < nb; ++blk) {
+      asm volatile("" : "+s"(track));  // one loop for both
+      store();                         // (the last block's again behind it)
+      load();
+      const bool is_sink = blk < sink_blocks;
+      if (is_sink ? blk < sink_see : blk >= see0 && blk < see1) {
+        const bool part = is_sink ? blk >= sink_full : blk < full0 || blk >= full1;
+        const int k0 = key0(blk), k1 = k0 + 32;
+        bool odd = false;
+        score(0);
+        if (part) mask(k0);
+        if (track || !started) follow();
+        if (track) odd = take_out();
+        accumulate();
+        if (track && odd) put_back(0, k0);
+        score(1);
+        if (part) {
+          if (!(k1 <= whi && k1 < len && (k1 + 31 > wlo - p.window || k1 < p.sinks))) goto done;
+          mask(k1);
+        }
+        if (track || !started) follow();
+        if (track) odd = take_out();
+        accumulate();
+        if (track && odd) put_back(1, k1);
+      }
+    done:
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kofs[i] ^= STAGE;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vofs[i] ^= STAGE;
       sync_step();
-      issue(I0{}, blk + 3);
-      compute(I1{}, blk + 1);
-      if (blk + 2 >= nb) break;
-      sync_step();
-      issue(I1{}, blk + 4);
-      compute(I2{}, blk + 2);
+    }
+    bool over = false;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int t = 0; t < 5; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) over |= !(fabsf(o[qt][t][i]) < 0x1p100f);
+    if (track || !__syncthreads_or(over)) break;
+    track = 1;
+    started = false;
+    clear();
+    // back to the first stage
+    if (nb & 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kofs[i] ^= STAGE;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vofs[i] ^= STAGE;
+    } else {
+      sofs ^= STAGE;
     }
   }
-  __builtin_amdgcn_s_waitcnt(0);       // no DMA into LDS outlives the workgroup
 
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -297,6 +401,7 @@ extern "C" int svla_attention_window_bf16(const void* q, int ldq, long q_bs, con
     return SVLA_EINVAL;
   if (ldq % 8 || ldk % 8 || ldv % 8 || ldo % 4 || q_bs % 8 || k_bs % 8 || v_bs % 8 || o_bs % 4)
     return SVLA_EINVAL;
+  if (ldk > (1 << 24) || ldv > (1 << 24)) return SVLA_EINVAL;   // offsets within a block: 32 bits
   if (ldq < hq * D || ldk < hkv * D || ldv < hkv * D || ldo < hq * D) return SVLA_EINVAL;
   if (!svla_aligned16(q) || !svla_aligned16(k) || !svla_aligned16(v) || ((uintptr_t)o & 7))
     return SVLA_EINVAL;
@@ -315,10 +420,21 @@ extern "C" int svla_attention_window_bf16(const void* q, int ldq, long q_bs, con
   p.scale_log2 = scale * 1.4426950408889634f;
   hipStream_t s = (hipStream_t)stream;
   const long g2 = (long)((sq + 127) / 128) * hq * batch;
-  if (sq <= 64 || g2 < 512)
-    hipLaunchKernelGGL(window_kernel<1>, dim3((sq + 63) / 64, hq, batch), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL(window_kernel<2>, dim3((sq + 127) / 128, hq, batch), dim3(256), 0, s, p);
+  // 128 rows a workgroup share each key's LDS reads, 64 rows waste fewer keys at
+  // the ends of a short window and fill more of the chip (MI355X, 64 / 128 rows:
+  // 2 x 16384 x 15 heads, window 4096: 723 / 606 us; 8 x 2000 x 12, window 500:
+  // 69 / 77)
+  const int qt = g2 >= 512 && min(window, sk) >= 1024 ? 2 : 1;
+  p.row_blocks = (sq + 64 * qt - 1) / (64 * qt);
+  const long blocks = (long)p.row_blocks * hkv * batch;
+  if (blocks > (1L << 24)) return SVLA_EINVAL;
+  p.blocks = (int)blocks;
+  p.run = (int)max(1L, min(16L, blocks / 32));
+  const long runs = (blocks + p.run - 1) / p.run;
+  const long grid = (runs + 7) / 8 * 8 * p.run * (hq / hkv);
+  if (grid > 0x7fffffffL) return SVLA_EINVAL;
+  if (qt == 1) hipLaunchKernelGGL(window_kernel<1>, dim3(grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(window_kernel<2>, dim3(grid), dim3(256), 0, s, p);
   SVLA_CHECK_LAUNCH();
   return SVLA_OK;
 }

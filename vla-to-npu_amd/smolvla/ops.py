@@ -365,31 +365,32 @@ def action_out_euler(a, w, x_f32, dt, x_bf16=None, norm=None):
 
 # ------------------------------------------------------------- attention ---
 def _attention_window(q, k, v, out, hq, hkv, scale, window, sinks, lens, q_pos):
-    B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
+    B, Sq, Sk, device = q.shape[0], q.shape[1], k.shape[1], q.device
     if window is None:
         raise ValueError('attention: mask="window" needs window')
     if not q.is_cuda:
         raise ValueError("smolvla ops take GPU tensors (no CPU fallback)")
+    args = []
     for t, rows, heads in ((q, Sq, hq), (k, Sk, hkv), (v, Sk, hkv), (out, Sq, hq)):
-        if (t.dtype != BF16 or t.device != q.device or t.shape[:2] != (B, rows)
-                or t.shape[2] < heads * 64):
-            raise ValueError(f"attention: bf16 [{B}, {rows}, {heads * 64}] on {q.device} expected, "
+        b, r, w = t.shape
+        if b != B or r != rows or w < heads * 64 or t.dtype is not BF16 or t.device != device:
+            raise ValueError(f"attention: bf16 [{B}, {rows}, {heads * 64}] on {device} expected, "
                              f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,)
-                             or not lens.is_contiguous() or lens.device != q.device):
-        raise ValueError(f"attention: lens must be contiguous int32 [{B}] on {q.device}")
-
-    # (a stride that no index uses need not be a valid one)
-    def ld(t):
-        return t.stride(1) if t.shape[1] > 1 else (t.shape[2] + 7) // 8 * 8
-
-    def bs(t):
-        return t.stride(0) if B > 1 else 0
-
-    with torch.cuda.device(q.device):
-        _lib.call("svla_attention_window_bf16", _ptr(q), ld(q), bs(q), _ptr(k), ld(k), bs(k),
-                  _ptr(v), ld(v), bs(v), _ptr(out), ld(out), bs(out), B, Sq, Sk, hq, hkv, 64,
-                  float(scale), int(q_pos), _ptr(lens), int(window), int(sinks), _stream())
+        # (a stride that no index uses need not be a valid one)
+        sb, sr, _ = t.stride()
+        args += [t.data_ptr(), sr if r > 1 else (w + 7) // 8 * 8, sb if b > 1 else 0]
+    if lens is not None and (lens.dtype is not torch.int32 or lens.shape != (B,)
+                             or not lens.is_contiguous() or lens.device != device):
+        raise ValueError(f"attention: lens must be contiguous int32 [{B}] on {device}")
+    args += [B, Sq, Sk, hq, hkv, 64, float(scale), int(q_pos),
+             None if lens is None else lens.data_ptr(), int(window), int(sinks)]
+    if torch.cuda.current_device() == device.index:
+        _lib.call("svla_attention_window_bf16", *args,
+                  torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            _lib.call("svla_attention_window_bf16", *args,
+                      torch._C._cuda_getCurrentRawStream(device.index))
     return out
 
 
