@@ -549,7 +549,7 @@ int svla_attention_window_bf16(const void* q, int ldq, long q_bs, const void* k,
  * the first `sinks` and the last (at least ring - 31) are kept: the ring is a
  * whole number of 32-token records.  data: svla_kv_cache_bytes bytes, 16-byte
  * aligned, zeroed once before the first use (a record may be decoded before
- * every token of it was written).  state: [batch][2] int32, set by
+ * every token of it was written).  state: [batch][4] int32, set by
  * svla_kv_reset; state[b][0] is n.
  *
  * Values: 32 consecutive values of a row share a power of two 2^E, E in
@@ -601,12 +601,20 @@ int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void*
  * probabilities bf16, bf16 out.  Rows behind counts[b] are written as zeros.  A
  * sequence of which a position that the call needs has left the ring (or that
  * is lost, or holds fewer tokens than counts[b]) gives NaN.  scale > 0,
- * rows * hq <= 2^24.  scratch: svla_kv_attention_scratch bytes, 4-byte aligned,
+ * rows * hq <= 2^24.  scratch: svla_kv_attention_scratch bytes, 16-byte aligned,
  * of this call alone until it is done (NULL where that is 0). */
 long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window);
 int svla_kv_attention_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o,
                            int ldo, long o_bs, int rows, const int* counts, int hq, float scale,
                            int window, void* scratch, long scratch_bytes, svla_stream_t stream);
+
+/* svla_kv_append_bf16 of new rows and svla_kv_attention_bf16 of their queries,
+ * with the same results; a single row per sequence is written by the attention
+ * itself. */
+int svla_kv_step_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, const void* k,
+                      int ldk, long k_bs, const void* v, int ldv, long v_bs, void* o, int ldo,
+                      long o_bs, int rows, const int* counts, const int* at, int hq, float scale,
+                      int window, void* scratch, long scratch_bytes, svla_stream_t stream);
 
 /* ------------------------------------------------------- pre-processing --
  * Camera frames -> vision-encoder input: n uint8 RGB frames [h, w, 3]

@@ -38,13 +38,14 @@ namespace {
 constexpr int TOK = 32;                 // tokens of a record
 constexpr int kMaxPos = 1 << 30;        // positions stay below it
 constexpr int kLost = 0x7fffffff;
+constexpr int kMaxSplits = 256;
 
 template <int BITS> constexpr int kPart = TOK * D * BITS / 8;      // bytes of K (or V) codes
 template <int BITS> constexpr int kRec = 2 * kPart<BITS> + 128;
 
 struct Cache {
   uint8_t* data;
-  int* state;                           // [batch][2]: n, lo
+  int* state;                           // [batch][4]: n, lo, arrivals, -
   int heads, sinks, sink_tiles, ring_tiles;
 };
 
@@ -148,11 +149,15 @@ template <int BITS> __device__ __forceinline__ u32x2 encode8(u32x4 x, int byte) 
   return r;
 }
 
-// largest magnitude (bf16 bits) of 8 values, then of the 4 lanes of the block
-__device__ __forceinline__ unsigned block_top(u32x4 x) {
+// largest magnitude (bf16 bits) of 8 values, and of those of the 4 lanes of a block
+__device__ __forceinline__ unsigned top8(u32x4 x) {
   unsigned t = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) t = max(t, max(x[i] & 0x7fff, (x[i] >> 16) & 0x7fff));
+  return t;
+}
+__device__ __forceinline__ unsigned block_top(u32x4 x) {
+  unsigned t = top8(x);
   t = max(t, (unsigned)__shfl_xor((int)t, 1));
   return max(t, (unsigned)__shfl_xor((int)t, 2));
 }
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int b = blockIdx.y;
-  const int n_old = c.state[2 * b], lo_old = c.state[2 * b + 1];
+  const int n_old = c.state[4 * b], lo_old = c.state[4 * b + 1];
   const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
   const Span sp = write_span(c, n_old, lo_old, a.at ? a.at[b] : n_old, count);
   Tiles t = tiles_of(c, sp.p0, sp.lo == kLost ? sp.p0 : sp.p0 + count);
@@ -259,8 +264,8 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
   if (whole) {
     __syncthreads();                    // every wave has read the old state
     if (threadIdx.x == 0) {
-      c.state[2 * b] = sp.n;
-      c.state[2 * b + 1] = sp.lo;
+      c.state[4 * b] = sp.n;
+      c.state[4 * b + 1] = sp.lo;
     }
   }
 }
@@ -268,16 +273,16 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
 __global__ void advance_kernel(AppendArgs a, int batch) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= batch) return;
-  const int n = a.c.state[2 * b];
+  const int n = a.c.state[4 * b];
   const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
-  const Span s = write_span(a.c, n, a.c.state[2 * b + 1], a.at ? a.at[b] : n, count);
-  a.c.state[2 * b] = s.n;
-  a.c.state[2 * b + 1] = s.lo;
+  const Span s = write_span(a.c, n, a.c.state[4 * b + 1], a.at ? a.at[b] : n, count);
+  a.c.state[4 * b] = s.n;
+  a.c.state[4 * b + 1] = s.lo;
 }
 
 __global__ void reset_kernel(int* state, int batch) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < 2 * batch) state[i] = 0;
+  if (i < 4 * batch) state[i] = 0;
 }
 
 // --------------------------------------------------------------- decoding ---
@@ -336,6 +341,89 @@ template <int BITS> struct Rec {
     return BITS == 4 ? u32x2{v[0][td], 0u}
                      : u32x2{v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2], v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2 + 1]};
   }
+  __device__ __forceinline__ void store(uint8_t* p, int lane) const {
+    constexpr int PART = kPart<BITS>;
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) {
+      *(u32x4*)(p + i * 1024 + lane * 16) = k[i];
+      *(u32x4*)(p + PART + i * 1024 + lane * 16) = v[i];
+    }
+    if (lane < 16) *(unsigned*)(p + 2 * PART + lane * 4) = ks;
+    if ((lane & 15) == 0) *(u32x4*)(p + 2 * PART + 64 + (lane >> 4) * 16) = vs;
+  }
+  // Token `slot` (the same in every lane) becomes the row kn, vn; the first
+  // token of a record clears it.
+  __device__ __forceinline__ void insert(const bf16* kn, const bf16* vn, int slot, int lane) {
+    const int grp = lane >> 4, col = lane & 15, half = slot >> 4, s16 = slot & 15;
+    if (slot == 0) {
+#pragma unroll
+      for (int i = 0; i < BITS / 4; ++i) k[i] = v[i] = u32x4{0, 0, 0, 0};
+      ks = 0;
+      vs = u32x4{0, 0, 0, 0};
+    }
+    auto put = [](unsigned& w, unsigned x, int shift, unsigned width) {
+      const unsigned m = width << shift;
+      w = (w & ~m) | ((x << shift) & m);
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32x4 x = *(const u32x4*)(kn + s * 32 + grp * 8);
+      unsigned top = top8(x);
+      top = max(top, (unsigned)__shfl_xor((int)top, 16));
+      top = max(top, (unsigned)__shfl_xor((int)top, 32));
+      const int byte = scale_byte<BITS>(top);
+      const u32x2 code = encode8<BITS>(x, byte);
+      if (col == s16) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          if (hf == half) {
+            if constexpr (BITS == 4) {
+              k[0][hf * 2 + s] = code[0];
+            } else {
+              k[hf][s * 2] = code[0];
+              k[hf][s * 2 + 1] = code[1];
+            }
+          }
+        put(ks, byte, 8 * (half * 2 + s), 255u);
+      }
+    }
+    const int j = half * 4 + (slot & 3);
+    const unsigned short* vb = reinterpret_cast<const unsigned short*>(vn);
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const u32x4 x = {(unsigned)vb[blk * 32 + col] | (unsigned)vb[blk * 32 + 16 + col] << 16, 0u, 0u, 0u};
+      unsigned top = top8(x);
+#pragma unroll
+      for (int m = 1; m < 16; m <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, m));
+      const int byte = scale_byte<BITS>(top);
+      const u32x2 code = encode8<BITS>(x, byte);
+      if (grp == (s16 >> 2)) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if constexpr (BITS == 4) {
+            unsigned y = v[0][2 * blk + w];
+            put(y, code[0] >> (4 * w), 4 * j, 15u);
+            v[0][2 * blk + w] = y;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (q == half) {
+                unsigned y = v[blk][2 * w + q];
+                put(y, code[0] >> (8 * w), 8 * (j & 3), 255u);
+                v[blk][2 * w + q] = y;
+              }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (q == half) {
+            unsigned y = vs[blk * 2 + q];
+            put(y, byte, 8 * (j & 3), 255u);
+            vs[blk * 2 + q] = y;
+          }
+      }
+    }
+  }
   template <int HALF, int S> __device__ __forceinline__ bf16x8 kfrag() const {
     return decode8<BITS>(kw(HALF, S), scale_of<HALF * 2 + S>(ks));
   }
@@ -363,7 +451,7 @@ __global__ __launch_bounds__(64) void read_kernel(ReadArgs a) {
   const Cache& c = a.c;
   const int lane = threadIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int grp = lane >> 4, col = lane & 15;
-  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
+  const int n = c.state[4 * b], lo = c.state[4 * b + 1];
   // (positions past kMaxPos do not exist; a start out of range reads zeros)
   const int first = min(max(a.starts ? a.starts[b] : a.start, -kMaxPos), kMaxPos - 1);
   const int p0 = max(first, 0), p1 = first + a.rows;
@@ -419,159 +507,230 @@ struct AttendArgs {
   bf16* o;
   long ldo, o_bs;
   const int* counts;
-  int rows, group, hq, window;
+  int rows, group, window;
   float scale_log2;
   int splits;
-  float* part;                          // [batch * heads][columns][splits][D + 2]
+  float *part, *stat;         // [batch * heads][columns][splits] x 64 and x 2
+  // one new row per sequence to be written on the way (NULL: none)
+  const bf16 *k, *v;
+  long k_bs, v_bs;
+  const int* at;
 };
+
+// What a call sees of one sequence.
+struct View {
+  int first, count;           // position of query row 0, rows
+  bool lost;                  // a position that the call needs is gone
+};
+__device__ __forceinline__ View view_of(const AttendArgs& a, int b, int n, int lo) {
+  View v;
+  v.count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
+  v.first = n - v.count;
+  const int need = max(a.c.sinks, a.window ? v.first - a.window + 1 : 0);
+  v.lost = lo == kLost || v.first < 0 || (need < n && (need - a.c.sinks) >> 5 < lo);
+  return v;
+}
+
+// Output of one column: 4 depths from d on; rows behind the count are zeros.
+__device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View& v, int r) {
+  const float inv = l > 0.f ? 1.0f / l : l;        // nothing visible: 0; NaN stays
+  bf16x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = f2bf(r >= v.count ? 0.f : v.lost ? __builtin_nanf("") : o[i] * inv);
+  *reinterpret_cast<bf16x4*>(out) = y;
+}
 
 // Columns: column j of a KV head is query row j / group of query head
 // j % group of the head's group, so all the query heads that share a KV head
-// share each record that a wave decodes.  A wave holds QT tiles of 16 columns;
-// KW of the workgroup's 4 waves take turns at the records of the same columns
-// and are joined through LDS, the others hold further columns.  The records of
-// a call are split over blockIdx.y too when there are few columns; the parts
-// (running maximum, sum and unscaled output) are then joined by join_kernel.
+// share each record that a wave decodes.  A workgroup holds QT tiles of 16
+// columns; its 4 waves take turns at the records and are joined through LDS.
+// The records of a call are split over blockIdx.y too when there are few
+// columns; the parts (reference, sum, unscaled output) are then joined by
+// join_kernel.
 //
 // S^T[token, column] = K . Q^T and O^T[d, column] = V^T . P^T, so a lane owns
 // one column (lane & 15); the accumulators of S^T are the operand P^T as they
-// stand.  The maximum moves only when a score passes it by 2^8 (exp2 units).
-// The sum of the rounded probabilities is an MFMA with a row of ones.
-template <int BITS, int QT, int KW>
-__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
-  constexpr int NQ = 4 / KW;                       // column groups of a workgroup
-  __shared__ float s_part[KW > 1 ? NQ * (KW - 1) * QT * 16 * (D + 2) : 1];
+// stand.  The sum of the rounded probabilities is an MFMA with a row of ones.
+//
+// Only the first tokens set the maximum: any reference gives the same quotient
+// as long as nothing overflows.  Where something does (scores over 2^100 times
+// the first ones, V that large or NaN: also behind the mask, as 0 * NaN), the
+// wave goes over its records once more, following the maximum, and a column
+// then meets only what it sees, NaN blocks apart.
+//
+// PF records are in registers or on their way to them.
+template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2) : 8 / BITS;
+
+// NEW: one new row per sequence is written on the way.
+template <int BITS, int QT, bool NEW>
+__global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs a) {
+  constexpr int PF = kAhead<BITS, QT>, KW = 4, LD = 16 * QT + 1;
+  __shared__ float s_part[KW - 1][D + 2][LD];      // per wave: 64 depths, reference, sum
   const Cache& c = a.c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = lane >> 4, col = lane & 15;
   const int b = blockIdx.z / c.heads, h = blockIdx.z - b * c.heads;
-  const int kw = wave % KW, cg = wave / KW;
   const int ncol = a.rows * a.group;
-  const int col0 = (blockIdx.x * NQ + cg) * QT * 16;
-  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
-  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
-  const int first = n - count;                     // position of query row 0
-  // the whole call needs positions from `need`; NaN when some are gone
-  const int need = max(c.sinks, a.window ? first - a.window + 1 : 0);
-  const bool lost = lo == kLost || first < 0 || (n > c.sinks && (need - c.sinks) >> 5 < lo && need < n);
+  const int col0 = blockIdx.x * QT * 16;
+  Span span = {0, c.state[4 * b], c.state[4 * b + 1]};
+  if constexpr (NEW) {
+    const int add = a.counts ? min(max(a.counts[b], 0), 1) : 1;
+    span = write_span(c, span.n, span.lo, a.at ? a.at[b] : span.n, add);
+  }
+  const View view = view_of(a, b, span.n, span.lo);
+  const int first = view.first, count = view.count;
 
   int qpos[QT];                                    // of this lane's column; -1: none
-  const bf16* qrow[QT];
   bf16x8 qf[QT][2];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int j = min(col0 + t * 16 + col, ncol - 1);
     const int r = j / a.group, hh = h * a.group + j - r * a.group;
-    qpos[t] = r < count && col0 + t * 16 + col < ncol ? first + r : -1;
-    qrow[t] = a.q + b * a.q_bs + r * a.ldq + hh * D;
+    qpos[t] = r < count ? first + r : -1;
+    const bf16* q = a.q + b * a.q_bs + r * a.ldq + hh * D;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) qf[t][s] = ld8(qrow[t] + s * 32 + grp * 8);
+    for (int s = 0; s < 2; ++s) qf[t][s] = ld8(q + s * 32 + grp * 8);
   }
-  // positions of the wave's first and last column (ascending by column)
-  const int r0 = col0 / a.group, r1 = min(min(col0 + QT * 16, ncol) - 1, ncol - 1) / a.group;
+  // positions of the workgroup's first and last row
+  const int r0 = col0 / a.group, r1 = (min(col0 + QT * 16, ncol) - 1) / a.group;
   const int qlo = first + min(r0, count - 1), qhi = first + min(r1, count - 1);
-  const bool any = r0 < count && col0 < ncol && !lost;
 
   f32x4 o[QT][5];
-  float m_run[QT], m_thr[QT], m_off[QT];
+  float m_run[QT], m_off[QT];
   const float cs = a.scale_log2;
+  auto clear = [&]() {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
+    for (int t = 0; t < QT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m_run[t] = -INFINITY;
-    m_thr[t] = -INFINITY;
-    m_off[t] = 0.f;
-  }
+      for (int i = 0; i < 5; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[t] = -INFINITY;
+      m_off[t] = 0.f;
+    }
+  };
+  clear();
   bf16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.0f);
 
-  if (any) {
+  if (r0 < count && !view.lost) {
     const int wlo = a.window ? max(0, qlo - a.window + 1) : 0;
     // records: the sinks that some column sees, then the ring from `wlo`
     const int ns = (min(c.sinks, qhi + 1) + TOK - 1) / TOK;
     const int u0 = max(wlo - c.sinks, 0) >> 5;
     const int nr = qhi >= c.sinks ? max(((qhi - c.sinks) >> 5) - u0 + 1, 0) : 0;
     const int total = ns + nr;
-    const int per = (total + a.splits - 1) / a.splits;
+    const int per = max((total + a.splits - 1) / a.splits, min(KW * 4, total));
     const int t0 = blockIdx.y * per, t1 = min(total, t0 + per);
+    const int from = t0 + kw;
     const uint8_t* base = c.data + record(c, b, h, 0) * kRec<BITS>;
+    // record of place ti in the list (past the end: the last one)
+    int at_u = u0 % c.ring_tiles;
     auto addr = [&](int ti) {
-      const int u = ti < ns ? ti : c.sink_tiles + (u0 + ti - ns) % c.ring_tiles;
+      ti = min(ti, t1 - 1);
+      int u = ti;
+      if (ti >= ns) {
+        u = at_u + ti - ns;                        // < 2 ring_tiles: nr <= ring_tiles
+        u = c.sink_tiles + (u >= c.ring_tiles ? u - c.ring_tiles : u);
+      }
       return base + (long)u * kRec<BITS>;
     };
-    Rec<BITS> r;
-    if (t0 + kw < t1) r.load(addr(t0 + kw), lane);
-    for (int ti = t0 + kw; ti < t1; ti += KW) {
-      Rec<BITS> nx;
-      nx.load(addr(min(ti + KW, t1 - 1)), lane);
+    int track = 0;             // follow the maximum at every record
+    bool started = false;      // every column of the wave has seen a token
+    // One record.  FOLLOW: the maximum moves and, from the second time over the
+    // records on, columns meet only what they see.
+    auto step = [&](auto FOLLOW, Rec<BITS>& r, int ti) __attribute__((always_inline)) {
       const bool sink = ti < ns;
       const int pos0 = sink ? ti * TOK : c.sinks + (u0 + ti - ns) * TOK;
-      const int plim = sink ? c.sinks : kMaxPos;
-      // all 32 positions are visible to every column of the wave
+      const int plim = sink ? c.sinks : kMaxPos;    // (positions of the ring are no sinks)
+      // all 32 positions are visible to every column of the workgroup
       const bool full = pos0 + TOK - 1 <= qlo && pos0 + TOK <= plim &&
                         (!a.window || pos0 > qhi - a.window || pos0 + TOK <= c.sinks);
-      const bf16x8 k00 = r.template kfrag<0, 0>(), k01 = r.template kfrag<0, 1>();
-      const bf16x8 k10 = r.template kfrag<1, 0>(), k11 = r.template kfrag<1, 1>();
       f32x4 sc[QT][2];
+      {
+        const bf16x8 k00 = r.template kfrag<0, 0>(), k01 = r.template kfrag<0, 1>();
+        const bf16x8 k10 = r.template kfrag<1, 0>(), k11 = r.template kfrag<1, 1>();
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k00, qf[t][0], x, 0, 0, 0);
-        y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k10, qf[t][0], y, 0, 0, 0);
-        sc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k01, qf[t][1], x, 0, 0, 0);
-        sc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k11, qf[t][1], y, 0, 0, 0);
+        for (int t = 0; t < QT; ++t) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+          x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k00, qf[t][0], x, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k10, qf[t][0], y, 0, 0, 0);
+          sc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k01, qf[t][1], x, 0, 0, 0);
+          sc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k11, qf[t][1], y, 0, 0, 0);
+        }
       }
-      auto sees = [&](int t, int half, int i) {
-        const int p = pos0 + half * 16 + grp * 4 + i;
-        return p <= qpos[t] && p < plim && (!a.window || p > qpos[t] - a.window || p < c.sinks);
+      auto sees = [&](int t, int i) {               // token (i >> 2) * 16 + 4 grp + (i & 3)
+        const int before = !sink && a.window ? qpos[t] - a.window : -1;
+        const int n = min(qpos[t], plim - 1) - before;          // (before, before + n]
+        return (unsigned)(pos0 + grp * 4 - before - 1 + (i >> 2) * 16 + (i & 3)) < (unsigned)n;
       };
-      bool nanfix = false;
-      u32x4 vs = r.vs;
       if (!full) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            sc[t][i >> 2][i & 3] = sees(t, i >> 2, i & 3) ? sc[t][i >> 2][i & 3] : -INFINITY;
-        // a NaN block of a token that some column does not see must not reach
-        // that column through 0 * NaN: look for scale bytes 0xff
-        unsigned bad = 0;
+            sc[t][i >> 2][i & 3] = sees(t, i) ? sc[t][i >> 2][i & 3] : -INFINITY;
+      }
+      if constexpr (decltype(FOLLOW)::value) {
+        // the maximum moves when a score passes it by 2^8 (exp2 units)
+        bool seen_all = true;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= (~vs[i] - 0x01010101u) & vs[i] & 0x80808080u;
-        nanfix = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-        if (nanfix)
+        for (int t = 0; t < QT; ++t) {
+          float mx = sc[t][0][0];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // (bytes never exceed 253 otherwise: 0xff is the only one with
-            // its lowest two bits and all others set)
-            unsigned w = 0;
+          for (int i = 1; i < 8; ++i) mx = smax(mx, sc[t][i >> 2][i & 3]);
+          mx = max_xor32(max_xor16(mx));
+          const bool grow = mx * cs > m_run[t] * cs + 8.f;
+          if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float m_new = smax(m_run[t], mx);
+            const float alpha = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m_new) * cs);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const unsigned x = (vs[i] >> (8 * e)) & 255u;
-              w |= (x == 255u ? 127u : x) << (8 * e);
-            }
-            r.vs[i] = w;
+            for (int i = 0; i < 5; ++i) o[t][i] *= alpha;
+            m_run[t] = m_new;
+            m_off[t] = m_new == -INFINITY ? 0.f : -m_new * cs;
           }
+          seen_all = seen_all && (m_run[t] != -INFINITY || qpos[t] < 0);
+        }
+        started = __builtin_amdgcn_ballot_w64(!seen_all) == 0;
+      }
+      if (decltype(FOLLOW)::value && track) {
+        // NaN blocks (scale byte 0xff) count as 0 in V and are added to the
+        // columns that see them
+#pragma unroll 1
+        for (int blk = 0; blk < 2; ++blk) {
+          const unsigned v0 = blk ? r.vs[2] : r.vs[0], v1 = blk ? r.vs[3] : r.vs[1];
+          unsigned nan_bits = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            nan_bits |= ((((j < 4 ? v0 : v1) >> (8 * (j & 3))) & 255u) == 255u ? 1u : 0u) << j;
+          if (!__builtin_amdgcn_ballot_w64(nan_bits != 0)) continue;
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            bf16x8 pn;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              pn[j] = f2bf(((nan_bits >> j) & 1u) && sees(t, j) ? __builtin_nanf("") : 0.f);
+            f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pn, z, 0, 0, 0);
+#pragma unroll
+            for (int td = 0; td < 4; ++td)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[t][td][i] += (td >> 1) == blk ? z[i] : 0.f;
+          }
+          unsigned w0 = 0, w1 = 0;               // bytes 0xff: any valid scale
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w0 |= ((nan_bits >> j) & 1u ? 0x80u : 0u) << (8 * j);
+            w1 |= ((nan_bits >> (4 + j)) & 1u ? 0x80u : 0u) << (8 * j);
+          }
+          r.vs[0] ^= blk ? 0u : w0;
+          r.vs[1] ^= blk ? 0u : w1;
+          r.vs[2] ^= blk ? w0 : 0u;
+          r.vs[3] ^= blk ? w1 : 0u;
+        }
       }
       bf16x8 pf[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        float mx = sc[t][0][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = smax(mx, sc[t][i >> 2][i & 3]);
-        mx = max_xor32(max_xor16(mx));
-        const bool grow = mx * cs > m_thr[t];
-        if (__builtin_amdgcn_ballot_w64(grow)) {
-          const float m_new = smax(m_run[t], mx);
-          const float alpha = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m_new) * cs);
-#pragma unroll
-          for (int i = 0; i < 5; ++i) o[t][i] *= alpha;
-          m_run[t] = m_new;
-          m_thr[t] = m_new * cs + 8.f;
-          m_off[t] = m_new == -INFINITY ? 0.f : -m_new * cs;
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           pf[t][i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t])));
@@ -584,118 +743,156 @@ __global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
         for (int t = 0; t < QT; ++t)
           o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[t][td], 0, 0, 0);
       }
-      if (nanfix) {
+    };
+    // the newest record, where the new row goes: its wave takes it first
+    const bool newest = NEW && t1 == total && kw == ((total - 1 - t0) & (KW - 1));
+    const int tend = newest ? t1 - 1 : t1;
+    while (from < t1) {
+      Rec<BITS> r0, r[PF];
+      int cur = newest ? total - 1 : from, ti = newest ? from : from + KW;
+      r0.load(addr(cur), lane);
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int blk = 0; blk < 2; ++blk) {
-            bf16x8 pn;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const bool isnan = ((vs[blk * 2 + (j >> 2)] >> (8 * (j & 3))) & 255u) == 255u;
-              pn[j] = f2bf(isnan && sees(t, j >> 2, j & 3) ? __builtin_nanf("") : 0.f);
-            }
-#pragma unroll
-            for (int td = blk * 2; td < blk * 2 + 2; ++td)
-              o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pn, o[t][td], 0, 0, 0);
-          }
+      for (int i = 0; i < PF; ++i) r[i].load(addr(ti + i * KW), lane);
+      if (newest) {
+        const int slot = (span.p0 < c.sinks ? span.p0 : span.p0 - c.sinks) & (TOK - 1);
+        r0.insert(a.k + b * a.k_bs + h * D, a.v + b * a.v_bs + h * D, slot, lane);
+        r0.store(const_cast<uint8_t*>(addr(cur)), lane);
       }
-      r = nx;
+      bool more = false;
+      for (;;) {
+        step(std::true_type{}, r0, cur);
+        if (ti >= tend || !(track || !started)) break;
+        cur = ti;
+        ti += KW;
+        r0.load(addr(cur), lane);
+        more = true;
+      }
+      if (more && ti < tend) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) r[i].load(addr(ti + i * KW), lane);
+      }
+      for (; ti < tend; ti += PF * KW) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+          if (ti + i * KW >= tend) break;
+          step(std::false_type{}, r[i], ti + i * KW);
+          r[i].load(addr(ti + (i + PF) * KW), lane);
+        }
+      }
+      bool over = false;
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) over |= !(fabsf(o[t][i][e]) < 0x1p100f);
+      if (track || !__builtin_amdgcn_ballot_w64(over)) break;
+      track = 1;
+      clear();
     }
   }
 
-  // join the KW waves of the same columns
-  if constexpr (KW > 1) {
-    if (kw > 0) {
-      float* sp = s_part + ((cg * (KW - 1) + kw - 1) * QT) * 16 * (D + 2);
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float* row = sp + (t * 16 + col) * (D + 2);
-#pragma unroll
-        for (int td = 0; td < 4; ++td)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) row[2 + td * 16 + grp * 4 + i] = o[t][td][i];
-        if (grp == 0) { row[0] = m_run[t]; row[1] = o[t][4][0]; }
-      }
-    }
-    __syncthreads();
-    if (kw > 0) return;
+  // join the waves
+  if (kw > 0) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float m = m_run[t];
-      for (int w = 0; w < KW - 1; ++w)
-        m = smax(m, s_part[((cg * (KW - 1) + w) * QT + t) * 16 * (D + 2) + col * (D + 2)]);
-      const float al = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m) * cs);
-#pragma unroll
-      for (int i = 0; i < 5; ++i) o[t][i] *= al;
-      for (int w = 0; w < KW - 1; ++w) {
-        const float* row = s_part + ((cg * (KW - 1) + w) * QT + t) * 16 * (D + 2) + col * (D + 2);
-        const float aw = row[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((row[0] - m) * cs);
-#pragma unroll
-        for (int td = 0; td < 4; ++td)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][td][i] += aw * row[2 + td * 16 + grp * 4 + i];
-        o[t][4][0] += aw * row[1];
-      }
-      m_run[t] = m;
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int j = col0 + t * 16 + col;
-    if (j >= ncol) continue;
-    if (a.splits > 1) {
-      float* row = a.part + (((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y) * (D + 2);
 #pragma unroll
       for (int td = 0; td < 4; ++td)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) row[2 + td * 16 + grp * 4 + i] = o[t][td][i];
-      if (grp == 0) { row[0] = m_run[t]; row[1] = o[t][4][0]; }
+        for (int i = 0; i < 4; ++i) s_part[kw - 1][td * 16 + grp * 4 + i][t * 16 + col] = o[t][td][i];
+      if (grp == 0) {
+        s_part[kw - 1][D][t * 16 + col] = m_run[t];
+        s_part[kw - 1][D + 1][t * 16 + col] = o[t][4][0];
+      }
+    }
+  }
+  __syncthreads();
+  if (kw > 0) {
+    // the last workgroup of a sequence to have read its state moves it on
+    if (NEW && threadIdx.x == 64) {
+      const int all = gridDim.y * c.heads;
+      if (__hip_atomic_fetch_add(&c.state[4 * b + 2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1) {
+        c.state[4 * b] = span.n;
+        c.state[4 * b + 1] = span.lo;
+        c.state[4 * b + 2] = 0;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int jj = t * 16 + col, j = col0 + jj;
+    float m = m_run[t];
+#pragma unroll
+    for (int w = 0; w < KW - 1; ++w) m = smax(m, s_part[w][D][jj]);
+    const float al = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m) * cs);
+    float l = o[t][4][0] * al;
+#pragma unroll
+    for (int td = 0; td < 4; ++td) o[t][td] *= al;
+#pragma unroll
+    for (int w = 0; w < KW - 1; ++w) {
+      const float mw = s_part[w][D][jj];
+      const float aw = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * cs);
+#pragma unroll
+      for (int td = 0; td < 4; ++td)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][td][i] += aw * s_part[w][td * 16 + grp * 4 + i][jj];
+      l += aw * s_part[w][D + 1][jj];
+    }
+    if (j >= ncol) continue;
+    if (a.splits > 1) {
+      const long at = ((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y;
+#pragma unroll
+      for (int td = 0; td < 4; ++td) *(f32x4*)(a.part + at * D + td * 16 + grp * 4) = o[t][td];
+      if (grp == 0) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
       continue;
     }
     const int r = j / a.group, hh = h * a.group + j - r * a.group;
-    const float l = o[t][4][0];
-    float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a NaN sum stays one)
-    if (r >= count) inv = 0.f;
-    bf16* out = a.o + b * a.o_bs + r * a.ldo + hh * D;
 #pragma unroll
-    for (int td = 0; td < 4; ++td) {
-      bf16x4 y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        y[i] = f2bf(r >= count ? 0.f : lost ? __builtin_nanf("") : o[t][td][i] * inv);
-      *reinterpret_cast<bf16x4*>(out + td * 16 + grp * 4) = y;
-    }
+    for (int td = 0; td < 4; ++td)
+      put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + td * 16 + grp * 4, o[t][td], l, view, r);
   }
 }
 
-// One wave per column: joins the parts of the splits.
+// Joins the parts of the splits: a workgroup per column, its 16 groups of 16
+// lanes (4 depths a lane) take turns at the parts.
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+  __shared__ float s_w[kMaxSplits];
+  __shared__ f32x4 s_o[4][16];
   const Cache& c = a.c;
-  const int lane = threadIdx.x & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int ncol = a.rows * a.group;
-  const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (j >= ncol) return;
+  const int j = blockIdx.x;
   const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
-  const int n = c.state[2 * b], lo = c.state[2 * b + 1];
-  const int count = a.counts ? min(max(a.counts[b], 0), a.rows) : a.rows;
-  const int first = n - count;
-  const int need = max(c.sinks, a.window ? first - a.window + 1 : 0);
-  const bool lost = lo == kLost || first < 0 || (n > c.sinks && (need - c.sinks) >> 5 < lo && need < n);
-  const int r = j / a.group, hh = h * a.group + j - r * a.group;
-  const float* row = a.part + ((long)blockIdx.y * ncol + j) * a.splits * (D + 2);
+  const long at = ((long)blockIdx.y * ncol + j) * a.splits;
+  // every wave: the weights of the parts and the sum
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = smax(m, row[s * (D + 2)]);
-  float l = 0.f, o = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = row + s * (D + 2);
-    const float w = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((p[0] - m) * a.scale_log2);
-    l += w * p[1];
-    o += w * p[2 + lane];
+  for (int s = lane; s < a.splits; s += 64) m = smax(m, a.stat[2 * (at + s)]);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) m = smax(m, __shfl_xor(m, x));
+  float l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) {
+    const float ms = a.stat[2 * (at + s)];
+    const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - m) * a.scale_log2);
+    l += w * a.stat[2 * (at + s) + 1];
+    if (wave == 0) s_w[s] = w;
   }
-  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-  a.o[b * a.o_bs + r * a.ldo + hh * D + lane] =
-      f2bf(r >= count ? 0.f : lost ? __builtin_nanf("") : o * inv);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+  __syncthreads();
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int d4 = (tid & 15) * 4;
+#pragma unroll 4
+  for (int s = tid >> 4; s < a.splits; s += 16) o += s_w[s] * *(const f32x4*)(a.part + (at + s) * D + d4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = xor32_sum(xor16_sum(o[i]));
+  if (lane < 16) s_o[wave][lane] = o;
+  __syncthreads();
+  if (tid >= 16) return;
+  o = s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid];
+  const View view = view_of(a, b, c.state[4 * b], c.state[4 * b + 1]);
+  const int r = j / a.group, hh = h * a.group + j - r * a.group;
+  put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + d4, o, l, view, r);
 }
 
 bool cache_ok(const svla_kv_cache* c) {
@@ -720,17 +917,8 @@ bool rows_ok(const void* p, int ld, long bs, int heads) {
   return p && svla_aligned16(p) && ld % 8 == 0 && bs % 8 == 0 && ld >= heads * D;
 }
 
-// splits of a call whose columns fill `wgs` workgroups of `kw` key waves over
-// at most `tiles` records
-int pick_splits(long wgs, int kw, long tiles) {
-  const long per_wave = 8;                       // records that a wave should get at least
-  long s = (2 * 256 + wgs - 1) / wgs;
-  s = min(s, (tiles + kw * per_wave - 1) / (kw * per_wave));
-  return (int)max(1L, min(s, 128L));
-}
-
 struct Plan {
-  int qt, kw, splits;
+  int qt, splits;
   dim3 grid;
 };
 
@@ -738,16 +926,73 @@ Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   Plan p;
   const long ncol = (long)rows * (hq / c->n_kv_heads);
   const long bh = (long)c->batch * c->n_kv_heads;
-  p.qt = 1;
-  p.kw = ncol <= 16 ? 4 : 1;
-  const int nq = 4 / p.kw;
-  const long cols = 16L * p.qt * nq;
-  const long x = (ncol + cols - 1) / cols;
+  p.qt = ncol <= 16 ? 1 : ncol <= 32 ? 2 : 4;
+  const long x = (ncol + 16 * p.qt - 1) / (16 * p.qt);
+  // records of a sequence, at most; a wave should have 4 of them
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
   const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
-  p.splits = p.kw == 4 ? pick_splits(x * bh, p.kw, tiles) : 1;
+  const long want = 1024 / p.qt;
+  p.splits = (int)max(1L, min(min((want + x * bh - 1) / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
   p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
   return p;
+}
+
+long scratch_of(const svla_kv_cache* c, const Plan& p, int rows, int hq) {
+  return p.splits > 1 ? (long)c->batch * hq * rows * p.splits * (D + 2) * 4 : 0;
+}
+
+template <int BITS>
+void launch_attend(const Plan& p, const AttendArgs& a, hipStream_t s) {
+  if (a.k) {
+    if (p.qt == 1) hipLaunchKernelGGL((attend_kernel<BITS, 1, true>), p.grid, dim3(256), 0, s, a);
+    else if (p.qt == 2) hipLaunchKernelGGL((attend_kernel<BITS, 2, true>), p.grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<BITS, 4, true>), p.grid, dim3(256), 0, s, a);
+  } else {
+    if (p.qt == 1) hipLaunchKernelGGL((attend_kernel<BITS, 1, false>), p.grid, dim3(256), 0, s, a);
+    else if (p.qt == 2) hipLaunchKernelGGL((attend_kernel<BITS, 2, false>), p.grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<BITS, 4, false>), p.grid, dim3(256), 0, s, a);
+  }
+}
+
+// Checks a call's arguments and lays out its plan; rows == 0: no more than that.
+int attend_args(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o, int ldo,
+                long o_bs, int rows, const int* counts, int hq, float scale, int window,
+                void* scratch, long scratch_bytes, Plan* p, AttendArgs* a) {
+  if (!cache_ok(c) || rows < 0 || hq <= 0 || hq % c->n_kv_heads || window < 0 ||
+      !(scale > 0.f) || !(scale < 1e30f))
+    return SVLA_EINVAL;
+  if (rows == 0) return SVLA_OK;
+  if ((long)rows * hq > (1L << 24)) return SVLA_EINVAL;
+  if (!rows_ok(q, ldq, q_bs, hq) || !o || ((uintptr_t)o & 7) || ldo % 4 || o_bs % 4 || ldo < hq * D)
+    return SVLA_EINVAL;
+  *p = plan_attend(c, rows, hq, window);
+  if (scratch_of(c, *p, rows, hq) > scratch_bytes ||
+      (p->splits > 1 && (!scratch || !svla_aligned16(scratch))))
+    return SVLA_EINVAL;
+  *a = AttendArgs{};
+  a->c = device_cache(c);
+  a->q = static_cast<const bf16*>(q); a->ldq = ldq; a->q_bs = q_bs;
+  a->o = static_cast<bf16*>(o); a->ldo = ldo; a->o_bs = o_bs;
+  a->counts = counts;
+  a->rows = rows;
+  a->group = hq / c->n_kv_heads;
+  a->window = min(window, kMaxPos);
+  a->scale_log2 = scale * 1.4426950408889634f;
+  a->splits = p->splits;
+  a->part = static_cast<float*>(scratch);
+  a->stat = a->part + (long)c->batch * hq * rows * p->splits * D;
+  return SVLA_OK;
+}
+
+int run_attend(const svla_kv_cache* c, const Plan& p, const AttendArgs& a, hipStream_t s) {
+  if (c->format == SVLA_KV_MXFP4) launch_attend<4>(p, a, s);
+  else launch_attend<8>(p, a, s);
+  SVLA_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    hipLaunchKernelGGL(join_kernel, dim3(a.rows * a.group, p.grid.z), dim3(256), 0, s, a);
+    SVLA_CHECK_LAUNCH();
+  }
+  return SVLA_OK;
 }
 
 }  // namespace
@@ -763,7 +1008,7 @@ long svla_kv_cache_bytes(int batch, int n_kv_heads, int head_dim, int format, in
 
 int svla_kv_reset(const svla_kv_cache* c, svla_stream_t stream) {
   if (!cache_ok(c)) return SVLA_EINVAL;
-  hipLaunchKernelGGL(reset_kernel, dim3((2 * c->batch + 255) / 256), dim3(256), 0,
+  hipLaunchKernelGGL(reset_kernel, dim3((4 * c->batch + 255) / 256), dim3(256), 0,
                      (hipStream_t)stream, c->state, c->batch);
   SVLA_CHECK_LAUNCH();
   return SVLA_OK;
@@ -830,52 +1075,41 @@ int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void*
 
 long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window) {
   if (!cache_ok(c) || rows <= 0 || hq <= 0 || hq % c->n_kv_heads || window < 0) return 0;
-  const Plan p = plan_attend(c, rows, hq, window);
-  return p.splits > 1 ? (long)c->batch * hq * rows * p.splits * (D + 2) * 4 : 0;
+  return scratch_of(c, plan_attend(c, rows, hq, window), rows, hq);
+}
+
+int svla_kv_step_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, const void* k,
+                      int ldk, long k_bs, const void* v, int ldv, long v_bs, void* o, int ldo,
+                      long o_bs, int rows, const int* counts, const int* at, int hq, float scale,
+                      int window, void* scratch, long scratch_bytes, svla_stream_t stream) {
+  Plan p;
+  AttendArgs a;
+  const int rc = attend_args(c, q, ldq, q_bs, o, ldo, o_bs, rows, counts, hq, scale, window, scratch,
+                             scratch_bytes, &p, &a);
+  if (rc) return rc;
+  if (rows > 0 && (!rows_ok(k, ldk, k_bs, c->n_kv_heads) || !rows_ok(v, ldv, v_bs, c->n_kv_heads)))
+    return SVLA_EINVAL;
+  // One new row, and one workgroup for all the columns of its record: written
+  // on the way (one token after 241 held, write + attention: 11.2 -> ... us)
+  if (rows != 1 || p.grid.x != 1) {
+    const int w = svla_kv_append_bf16(c, k, ldk, k_bs, v, ldv, v_bs, rows, counts, at, stream);
+    if (w || rows == 0) return w;
+  } else {
+    a.k = static_cast<const bf16*>(k); a.k_bs = k_bs;
+    a.v = static_cast<const bf16*>(v); a.v_bs = v_bs;
+    a.at = at;
+  }
+  return run_attend(c, p, a, (hipStream_t)stream);
 }
 
 int svla_kv_attention_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o,
                            int ldo, long o_bs, int rows, const int* counts, int hq, float scale,
                            int window, void* scratch, long scratch_bytes, svla_stream_t stream) {
-  if (!cache_ok(c) || rows < 0 || hq <= 0 || hq % c->n_kv_heads || window < 0 ||
-      !(scale > 0.f) || !(scale < 1e30f))
-    return SVLA_EINVAL;
-  if (rows == 0) return SVLA_OK;
-  if ((long)rows * hq > (1L << 24)) return SVLA_EINVAL;
-  if (!rows_ok(q, ldq, q_bs, hq) || !o || ((uintptr_t)o & 7) || ldo % 4 || o_bs % 4 || ldo < hq * D)
-    return SVLA_EINVAL;
-  const Plan p = plan_attend(c, rows, hq, window);
-  if (svla_kv_attention_scratch(c, rows, hq, window) > scratch_bytes ||
-      (p.splits > 1 && (!scratch || ((uintptr_t)scratch & 3))))
-    return SVLA_EINVAL;
+  Plan p;
   AttendArgs a;
-  a.c = device_cache(c);
-  a.q = static_cast<const bf16*>(q); a.ldq = ldq; a.q_bs = q_bs;
-  a.o = static_cast<bf16*>(o); a.ldo = ldo; a.o_bs = o_bs;
-  a.counts = counts;
-  a.rows = rows;
-  a.hq = hq;
-  a.group = hq / c->n_kv_heads;
-  a.window = min(window, kMaxPos);
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.splits = p.splits;
-  a.part = static_cast<float*>(scratch);
-  hipStream_t s = (hipStream_t)stream;
-  const bool f4 = c->format == SVLA_KV_MXFP4;
-  if (p.kw == 4) {
-    if (f4) hipLaunchKernelGGL((attend_kernel<4, 1, 4>), p.grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attend_kernel<8, 1, 4>), p.grid, dim3(256), 0, s, a);
-  } else {
-    if (f4) hipLaunchKernelGGL((attend_kernel<4, 1, 1>), p.grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attend_kernel<8, 1, 1>), p.grid, dim3(256), 0, s, a);
-  }
-  SVLA_CHECK_LAUNCH();
-  if (p.splits > 1) {
-    const dim3 grid((rows * a.group + 3) / 4, p.grid.z);
-    hipLaunchKernelGGL(join_kernel, grid, dim3(256), 0, s, a);
-    SVLA_CHECK_LAUNCH();
-  }
-  return SVLA_OK;
+  const int rc = attend_args(c, q, ldq, q_bs, o, ldo, o_bs, rows, counts, hq, scale, window, scratch,
+                             scratch_bytes, &p, &a);
+  return rc || rows == 0 ? rc : run_attend(c, p, a, (hipStream_t)stream);
 }
 
 }  // extern "C"

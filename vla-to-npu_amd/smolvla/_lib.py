@@ -116,6 +116,8 @@ SIGNATURES = {
     "svla_kv_read_bf16": [_kv, _p, _i, _l, _p, _i, _l, _i, _p, _i, _p],
     "svla_kv_attention_scratch": [_kv, _i, _i, _i],
     "svla_kv_attention_bf16": [_kv, _p, _i, _l, _p, _i, _l, _i, _p, _i, _f, _i, _p, _l, _p],
+    "svla_kv_step_bf16": [_kv, _p, _i, _l, _p, _i, _l, _p, _i, _l, _p, _i, _l, _i, _p, _p, _i, _f,
+                          _i, _p, _l, _p],
 }
 
 RESTYPES = {"svla_expert_workspace_size": ctypes.c_long,

@@ -27,28 +27,23 @@ from . import _lib
 
 BF16 = torch.bfloat16
 HEAD_DIM = 64
+SCALE = 1.0 / math.sqrt(HEAD_DIM)
 TOKENS = 32                     # tokens of a record
 FORMATS = {"mxfp4": 4, "mxfp8": 8}
 
 
-def _rows(name, t, batch, rows, width):
-    """A bf16 ``[B, T, >= width]`` GPU view with contiguous rows."""
+def _bad(name, t, batch, rows, width, device):
+    """Why ``t`` is no bf16 ``[batch, rows, >= width]`` view on the device."""
+    if not torch.is_tensor(t):
+        return f"{name}: a tensor expected"
     if not t.is_cuda:
-        raise ValueError("smolvla ops take GPU tensors (no CPU fallback)")
-    if t.dim() != 3 or t.dtype != BF16 or t.shape[0] != batch or t.shape[2] < width:
-        raise ValueError(f"{name}: bf16 [{batch}, rows, {width}] expected, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    if rows is not None and t.shape[1] != rows:
-        raise ValueError(f"{name}: {rows} rows expected, got {t.shape[1]}")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}: rows must be contiguous")
-    return t
-
-
-def _ld(t):
-    """(row stride, batch stride); a stride that no index uses is any valid one."""
-    width = (t.shape[2] + 7) // 8 * 8
-    return (t.stride(1) if t.shape[1] > 1 else width), (t.stride(0) if t.shape[0] > 1 else 0)
+        return "smolvla ops take GPU tensors (no CPU fallback)"
+    if t.device != device:
+        return f"{name} on {t.device}, cache on {device}"
+    if t.dim() == 3 and t.stride(2) != 1:
+        return f"{name}: rows must be contiguous"
+    return (f"{name}: bf16 [{batch}, {'rows' if rows is None else rows}, {width}] expected, got "
+            f"{t.dtype} {tuple(t.shape)}")
 
 
 class KVCache:
@@ -96,7 +91,7 @@ class KVCache:
         # (zeros: a record may be decoded before every token of it was written)
         self.data = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         self.device = self.data.device
-        self.state = torch.zeros(batch, 2, dtype=torch.int32, device=self.device)
+        self.state = torch.zeros(batch, 4, dtype=torch.int32, device=self.device)
         self._desc = _lib.KVCacheDesc(self.data.data_ptr(), self.state.data_ptr(), batch,
                                       n_kv_heads, HEAD_DIM, FORMATS[fmt], sinks, self.ring)
         self._ref = ctypes.byref(self._desc)
@@ -121,25 +116,38 @@ class KVCache:
                 raise RuntimeError(f"KVCache: sequences {over} hold more than {self.max_len} tokens")
 
     # ---------------------------------------------------------------- calls --
-    def _on(self, *tensors):
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"tensor on {t.device}, cache on {self.device}")
+    def _view(self, name, t, rows, width):
+        """(address, row stride, batch stride) of a bf16 ``[B, rows, >= width]``
+        view; a stride that no index uses is any valid one."""
+        try:
+            b, r, w = t.shape
+            sb, sr, sw = t.stride()
+            ok = (b == self.batch and (rows is None or r == rows) and w >= width and sw == 1
+                  and t.dtype is BF16 and t.device == self.device)
+        except (ValueError, AttributeError):
+            ok = False
+        if not ok:
+            raise ValueError(_bad(name, t, self.batch, rows, width, self.device))
+        return t.data_ptr(), (sr if r > 1 else (w + 7) // 8 * 8), (sb if b > 1 else 0)
+
+    def _new(self, rows, width):
+        return torch.empty((self.batch, rows, width), dtype=BF16, device=self.device)
 
     def _ints(self, name, t):
         if t is None:
             return None
-        if not torch.is_tensor(t) or t.dtype != torch.int32 or t.shape != (self.batch,) \
-                or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous int32 [{self.batch}] tensor expected")
-        self._on(t)
+        if not (torch.is_tensor(t) and t.dtype is torch.int32 and t.shape == (self.batch,)
+                and t.is_contiguous() and t.device == self.device):
+            raise ValueError(f"{name}: contiguous int32 [{self.batch}] tensor on {self.device} "
+                             "expected")
         return t.data_ptr()
 
     def _call(self, name, *args):
-        if torch.cuda.current_device() == self.device.index:
-            return _lib.call(name, self._ref, *args, torch.cuda.current_stream().cuda_stream)
-        with torch.cuda.device(self.device):
-            return _lib.call(name, self._ref, *args, torch.cuda.current_stream().cuda_stream)
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            return _lib.call(name, self._ref, *args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(index):
+            return _lib.call(name, self._ref, *args, torch._C._cuda_getCurrentRawStream(index))
 
     def reset(self):
         """Every sequence empty."""
@@ -151,11 +159,9 @@ class KVCache:
         ``[B]``; tokens behind it are taken back).  ``counts`` (int32 ``[B]``):
         how many of the rows are real."""
         width = self.n_kv_heads * HEAD_DIM
-        _rows("k", k, self.batch, None, width)
-        _rows("v", v, self.batch, k.shape[1], width)
-        self._on(k, v)
-        self._call("svla_kv_append_bf16", k.data_ptr(), *_ld(k), v.data_ptr(), *_ld(v),
-                   k.shape[1], self._ints("counts", counts), self._ints("at", at))
+        kv = self._view("k", k, None, width)
+        self._call("svla_kv_append_bf16", *kv, *self._view("v", v, k.shape[1], width), k.shape[1],
+                   self._ints("counts", counts), self._ints("at", at))
 
     def read(self, start=0, rows=None, k_out=None, v_out=None):
         """``(k, v)`` of positions ``start`` (an int, or int32 ``[B]``) to
@@ -165,20 +171,15 @@ class KVCache:
         if rows is None or rows < 0:
             raise ValueError("read: rows (a cache without max_len has no default)")
         width = self.n_kv_heads * HEAD_DIM
-        if k_out is None:
-            k_out = torch.empty(self.batch, rows, width, dtype=BF16, device=self.device)
-        if v_out is None:
-            v_out = torch.empty(self.batch, rows, width, dtype=BF16, device=self.device)
-        _rows("k_out", k_out, self.batch, rows, width)
-        _rows("v_out", v_out, self.batch, rows, width)
-        self._on(k_out, v_out)
+        k_out = self._new(rows, width) if k_out is None else k_out
+        v_out = self._new(rows, width) if v_out is None else v_out
+        kv = (*self._view("k_out", k_out, rows, width), *self._view("v_out", v_out, rows, width))
         starts = None
         if torch.is_tensor(start):
             starts, start = self._ints("start", start), 0
         elif start < 0:
             raise ValueError(f"start must not be negative, got {start}")
-        self._call("svla_kv_read_bf16", k_out.data_ptr(), *_ld(k_out), v_out.data_ptr(),
-                   *_ld(v_out), start, starts, rows)
+        self._call("svla_kv_read_bf16", *kv, start, starts, rows)
         return k_out, v_out
 
     def attend(self, q, n_heads, out=None, counts=None, scale=None):
@@ -186,31 +187,37 @@ class KVCache:
         n_heads * 64]``; with ``counts`` the last ``counts[b]``, rows behind
         them give zeros) over the cache: causal, within the cache's window and
         sinks.  A sequence of which needed tokens are gone gives NaN."""
+        return self._attend("svla_kv_attention_bf16", q, n_heads, (), out, counts, (), scale)
+
+    def step(self, q, k, v, n_heads, out=None, counts=None, at=None, scale=None):
+        """:meth:`append` of new rows and :meth:`attend` of their queries, in one
+        call (one launch less for a single row)."""
+        width = self.n_kv_heads * HEAD_DIM
+        if q.shape[1:2] != k.shape[1:2]:
+            raise ValueError("step: a query for every new row")
+        kv = (*self._view("k", k, None, width), *self._view("v", v, k.shape[1], width))
+        return self._attend("svla_kv_step_bf16", q, n_heads, kv, out, counts,
+                            (self._ints("at", at),), scale)
+
+    def _attend(self, name, q, n_heads, kv, out, counts, at, scale):
         width = n_heads * HEAD_DIM
-        _rows("q", q, self.batch, None, width)
+        qv = self._view("q", q, None, width)
         rows = q.shape[1]
         if self.max_rows is not None and rows > self.max_rows:
-            raise ValueError(f"attend: {rows} rows, the cache was made for {self.max_rows}")
+            raise ValueError(f"{rows} rows, the cache was made for {self.max_rows}")
         if out is None:
-            out = torch.empty(self.batch, rows, width, dtype=BF16, device=self.device)
-        _rows("out", out, self.batch, rows, width)
-        self._on(q, out)
-        window = self.window or 0
+            out = self._new(rows, width)
+            ov = (out.data_ptr(), width, rows * width)
+        else:
+            ov = self._view("out", out, rows, width)
         key = (rows, n_heads)
         nbytes = self._scratch.get(key)
         if nbytes is None:
             nbytes = self._scratch[key] = self._lib.svla_kv_attention_scratch(
-                self._ref, rows, n_heads, window)
-        scratch = (torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None)
-        scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale
-        self._call("svla_kv_attention_bf16", q.data_ptr(), *_ld(q), out.data_ptr(), *_ld(out),
-                   rows, self._ints("counts", counts), n_heads, scale, window,
+                self._ref, rows, n_heads, self.window or 0)
+        # (of this call alone: the allocator keeps it until the stream has passed)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        self._call(name, *qv, *kv, *ov, rows, self._ints("counts", counts), *at, n_heads,
+                   SCALE if scale is None else scale, self.window or 0,
                    scratch.data_ptr() if nbytes else None, nbytes)
         return out
-
-    def step(self, q, k, v, n_heads, out=None, counts=None, at=None, scale=None):
-        """:meth:`append` of new rows and :meth:`attend` of their queries."""
-        if q.shape[1] != k.shape[1]:
-            raise ValueError("step: a query for every new row")
-        self.append(k, v, counts=counts, at=at)
-        return self.attend(q, n_heads, out=out, counts=counts, scale=scale)
