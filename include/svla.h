@@ -501,6 +501,10 @@ int svla_rope(const void* x, int ldx, void* y, int ldy, int rows, int heads,
 int svla_rope_table(float* cos_t, float* sin_t, int max_pos, int head_dim, float theta,
                     svla_stream_t stream);
 
+/* The rows of the positions first .. first + rows - 1 (a stream's next tokens). */
+int svla_rope_table_at(float* cos_t, float* sin_t, int first, int rows, int head_dim, float theta,
+                       svla_stream_t stream);
+
 /* Transpose-pack a reference [K, N] (in x out) bf16 weight to [N, K]. */
 int svla_pack_weight_bf16(const void* w_kn, int ldw, void* out_nk, int k, int n,
                           svla_stream_t stream);

@@ -135,10 +135,10 @@ __global__ void rope_kernel(const void* __restrict__ x, long ldx, void* __restri
   }
 }
 
-__global__ void rope_table_kernel(float* ct, float* st, int max_pos, int half, float theta,
-                                  float two_over_d) {
+__global__ void rope_table_kernel(float* ct, float* st, int rows, int half, float theta,
+                                  float two_over_d, int first) {
   const int idx = blockIdx.x * blockDim.x + threadIdx.x;
-  if (idx < max_pos * half) rope_entry(ct, st, idx, half, theta, two_over_d);
+  if (idx < rows * half) rope_entry(ct, st, idx, half, theta, two_over_d, first);
 }
 
 __global__ void transpose_kernel(const bf16* __restrict__ w, long ldw, bf16* __restrict__ o,
@@ -271,15 +271,22 @@ int svla_rope(const void* x, int ldx, void* y, int ldy, int rows, int heads, con
   return SVLA_OK;
 }
 
-int svla_rope_table(float* cos_t, float* sin_t, int max_pos, int head_dim, float theta,
-                    svla_stream_t stream) {
-  if (max_pos <= 0 || head_dim <= 0 || head_dim % 2) return SVLA_EINVAL;
+int svla_rope_table_at(float* cos_t, float* sin_t, int first, int rows, int head_dim, float theta,
+                       svla_stream_t stream) {
+  if (first < 0 || rows <= 0 || first > 0x7fffffff - rows || head_dim <= 0 || head_dim % 2 ||
+      rows > 0x7fffff00 / (head_dim / 2))
+    return SVLA_EINVAL;
   const int half = head_dim / 2;
-  const int n = max_pos * half;
+  const int n = rows * half;
   hipLaunchKernelGGL(rope_table_kernel, dim3((n + 255) / 256), dim3(256), 0, (hipStream_t)stream,
-                     cos_t, sin_t, max_pos, half, theta, 2.0f / (float)head_dim);
+                     cos_t, sin_t, rows, half, theta, 2.0f / (float)head_dim, first);
   SVLA_CHECK_LAUNCH();
   return SVLA_OK;
+}
+
+int svla_rope_table(float* cos_t, float* sin_t, int max_pos, int head_dim, float theta,
+                    svla_stream_t stream) {
+  return svla_rope_table_at(cos_t, sin_t, 0, max_pos, head_dim, theta, stream);
 }
 
 int svla_pack_weight_bf16(const void* w_kn, int ldw, void* out_nk, int k, int n,

@@ -39,6 +39,7 @@ constexpr int TOK = 32;                 // tokens of a record
 constexpr int kMaxPos = 1 << 30;        // positions stay below it
 constexpr int kLost = 0x7fffffff;
 constexpr int kMaxSplits = 256;
+constexpr unsigned kMaxArrivals = 64;
 
 template <int BITS> constexpr int kPart = TOK * D * BITS / 8;      // bytes of K (or V) codes
 template <int BITS> constexpr int kRec = 2 * kPart<BITS> + 128;
@@ -168,11 +169,12 @@ __device__ __forceinline__ unsigned block_top(u32x4 x) {
 // codes are scattered as bytes, those of a token pair put together by the pair
 // of lanes l, l ^ 8 at 4 bits.  A record that keeps older tokens is read first.
 //
-// One workgroup per sequence where `whole` (its waves cover every record and
-// head, and it then stores the new state); else the records are spread over
-// blockIdx.x and advance_kernel stores the state.
+// The last workgroup of a sequence to have read its state stores the new one;
+// with more than kMaxArrivals of them advance_kernel does, since the arrivals at
+// one address take 6 ns each (4 x 32768 rows of 5 heads, 1280 workgroups a
+// sequence: 72 us against 39 + 4).
 template <int BITS>
-__global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
+__global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
   constexpr int PART = kPart<BITS>, REC = kRec<BITS>;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const Cache& c = a.c;
@@ -261,12 +263,12 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a, int whole) {
       for (int i = lane; i < REC / 16; i += 64) ((u32x4*)out)[i] = ((const u32x4*)rec)[i];
     __syncthreads();
   }
-  if (whole) {
-    __syncthreads();                    // every wave has read the old state
-    if (threadIdx.x == 0) {
-      c.state[4 * b] = sp.n;
-      c.state[4 * b + 1] = sp.lo;
-    }
+  __syncthreads();                      // every wave has read the old state
+  if (threadIdx.x == 0 && gridDim.x <= kMaxArrivals && __hip_atomic_fetch_add(&c.state[4 * b + 2], 1, __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1) {
+    c.state[4 * b] = sp.n;
+    c.state[4 * b + 1] = sp.lo;
+    c.state[4 * b + 2] = 0;
   }
 }
 
@@ -565,7 +567,7 @@ template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2)
 template <int BITS, int QT, bool NEW>
 __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs a) {
   constexpr int PF = kAhead<BITS, QT>, KW = 4, LD = 16 * QT + 1;
-  __shared__ float s_part[KW - 1][D + 2][LD];      // per wave: 64 depths, reference, sum
+  __shared__ float s_part[KW][D + 2][LD];          // per wave: 64 depths, reference, sum
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = lane >> 4, col = lane & 15;
@@ -792,65 +794,58 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
     }
   }
 
-  // join the waves
-  if (kw > 0) {
+  // join the waves: the 4 QT tiles (16 columns x 16 depths) are shared out
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
+  for (int t = 0; t < QT; ++t) {
 #pragma unroll
-      for (int td = 0; td < 4; ++td)
+    for (int td = 0; td < 4; ++td)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_part[kw - 1][td * 16 + grp * 4 + i][t * 16 + col] = o[t][td][i];
-      if (grp == 0) {
-        s_part[kw - 1][D][t * 16 + col] = m_run[t];
-        s_part[kw - 1][D + 1][t * 16 + col] = o[t][4][0];
-      }
+      for (int i = 0; i < 4; ++i) s_part[kw][td * 16 + grp * 4 + i][t * 16 + col] = o[t][td][i];
+    if (grp == 0) {
+      s_part[kw][D][t * 16 + col] = m_run[t];
+      s_part[kw][D + 1][t * 16 + col] = o[t][4][0];
     }
   }
   __syncthreads();
-  if (kw > 0) {
-    // the last workgroup of a sequence to have read its state moves it on
-    if (NEW && threadIdx.x == 64) {
-      const int all = gridDim.y * c.heads;
-      if (__hip_atomic_fetch_add(&c.state[4 * b + 2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1) {
-        c.state[4 * b] = span.n;
-        c.state[4 * b + 1] = span.lo;
-        c.state[4 * b + 2] = 0;
-      }
+  // the last workgroup of a sequence to have read its state moves it on
+  if (NEW && threadIdx.x == 64) {
+    const int all = gridDim.y * c.heads;
+    if (__hip_atomic_fetch_add(&c.state[4 * b + 2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1) {
+      c.state[4 * b] = span.n;
+      c.state[4 * b + 1] = span.lo;
+      c.state[4 * b + 2] = 0;
     }
-    return;
   }
+  const int jj = (QT == 1 ? 0 : QT == 2 ? kw >> 1 : kw) * 16 + col, j = col0 + jj;
+  float mw[KW], m = -INFINITY;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int jj = t * 16 + col, j = col0 + jj;
-    float m = m_run[t];
+  for (int w = 0; w < KW; ++w) {
+    mw[w] = s_part[w][D][jj];
+    m = smax(m, mw[w]);
+  }
+  float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < KW - 1; ++w) m = smax(m, s_part[w][D][jj]);
-    const float al = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[t] - m) * cs);
-    float l = o[t][4][0] * al;
+  for (int w = 0; w < KW; ++w) {
+    mw[w] = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw[w] - m) * cs);
+    l += mw[w] * s_part[w][D + 1][jj];
+  }
+  if (j >= ncol) return;
+  const int r = j / a.group, hh = h * a.group + j - r * a.group;
+  const long at = ((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y;
 #pragma unroll
-    for (int td = 0; td < 4; ++td) o[t][td] *= al;
+  for (int i = 0; i < QT; ++i) {
+    const int d = ((kw * QT + i) & 3) * 16 + grp * 4;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < KW - 1; ++w) {
-      const float mw = s_part[w][D][jj];
-      const float aw = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * cs);
+    for (int w = 0; w < KW; ++w)
 #pragma unroll
-      for (int td = 0; td < 4; ++td)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][td][i] += aw * s_part[w][td * 16 + grp * 4 + i][jj];
-      l += aw * s_part[w][D + 1][jj];
-    }
-    if (j >= ncol) continue;
-    if (a.splits > 1) {
-      const long at = ((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y;
-#pragma unroll
-      for (int td = 0; td < 4; ++td) *(f32x4*)(a.part + at * D + td * 16 + grp * 4) = o[t][td];
-      if (grp == 0) { a.stat[2 * at] = m; a.stat[2 * at + 1] = l; }
-      continue;
-    }
-    const int r = j / a.group, hh = h * a.group + j - r * a.group;
-#pragma unroll
-    for (int td = 0; td < 4; ++td)
-      put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + td * 16 + grp * 4, o[t][td], l, view, r);
+      for (int e = 0; e < 4; ++e) y[e] += mw[w] * s_part[w][d + e][jj];
+    if (a.splits > 1) *(f32x4*)(a.part + at * D + d) = y;
+    else put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + d, y, l, view, r);
+  }
+  if (a.splits > 1 && grp == 0 && (QT != 1 || kw == 0) && (QT != 2 || !(kw & 1))) {
+    a.stat[2 * at] = m;
+    a.stat[2 * at + 1] = l;
   }
 }
 
@@ -1034,15 +1029,15 @@ int svla_kv_append_bf16(const svla_kv_cache* c, const void* k, int ldk, long k_b
   tiles = min(tiles, (long)a.c.ring_tiles + a.c.sink_tiles);
   const long units = tiles * c->n_kv_heads;
   const size_t rec = c->format == SVLA_KV_MXFP4 ? kRec<4> : kRec<8>;
-  const bool whole = units <= 12;          // 12 records of 8 bits: 51 KB of LDS
-  const int waves = whole ? (int)units : 4;
-  const dim3 grid(whole ? 1 : (unsigned)min((units + 3) / 4, 1L << 20), c->batch);
+  // one workgroup per sequence up to 12 records (of 8 bits: 51 KB of LDS)
+  const int waves = units <= 12 ? (int)units : 4;
+  const dim3 grid((unsigned)min((units + waves - 1) / waves, 1L << 20), c->batch);
   if (c->format == SVLA_KV_MXFP4)
-    hipLaunchKernelGGL(append_kernel<4>, grid, dim3(64 * waves), waves * rec, s, a, (int)whole);
+    hipLaunchKernelGGL(append_kernel<4>, grid, dim3(64 * waves), waves * rec, s, a);
   else
-    hipLaunchKernelGGL(append_kernel<8>, grid, dim3(64 * waves), waves * rec, s, a, (int)whole);
+    hipLaunchKernelGGL(append_kernel<8>, grid, dim3(64 * waves), waves * rec, s, a);
   SVLA_CHECK_LAUNCH();
-  if (!whole) {
+  if (grid.x > kMaxArrivals) {
     hipLaunchKernelGGL(advance_kernel, dim3((c->batch + 255) / 256), dim3(256), 0, s, a, c->batch);
     SVLA_CHECK_LAUNCH();
   }

@@ -92,6 +92,7 @@ SIGNATURES = {
     "svla_silu_mul_bf16": [_p, _p, _p, _l, _p],
     "svla_rope": [_p, _i, _p, _i, _i, _i, _p, _p, _i, _i, _i, _p],
     "svla_rope_table": [_p, _p, _i, _i, _f, _p],
+    "svla_rope_table_at": [_p, _p, _i, _i, _i, _f, _p],
     "svla_pack_weight_bf16": [_p, _i, _p, _i, _i, _p],
     "svla_pack_gate_up_bf16": [_p, _p, _p, _i, _i, _p],
     "svla_embed_bf16": [_p, _p, _l, _i, _f, _p, _i, _l, _l, _i, _p],

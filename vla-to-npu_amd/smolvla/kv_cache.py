@@ -171,9 +171,16 @@ class KVCache:
         if rows is None or rows < 0:
             raise ValueError("read: rows (a cache without max_len has no default)")
         width = self.n_kv_heads * HEAD_DIM
-        k_out = self._new(rows, width) if k_out is None else k_out
-        v_out = self._new(rows, width) if v_out is None else v_out
-        kv = (*self._view("k_out", k_out, rows, width), *self._view("v_out", v_out, rows, width))
+        if k_out is None:
+            k_out = self._new(rows, width)
+            kv = (k_out.data_ptr(), width, rows * width)
+        else:
+            kv = self._view("k_out", k_out, rows, width)
+        if v_out is None:
+            v_out = self._new(rows, width)
+            kv += (v_out.data_ptr(), width, rows * width)
+        else:
+            kv += self._view("v_out", v_out, rows, width)
         starts = None
         if torch.is_tensor(start):
             starts, start = self._ints("start", start), 0
@@ -206,7 +213,7 @@ class KVCache:
         if self.max_rows is not None and rows > self.max_rows:
             raise ValueError(f"{rows} rows, the cache was made for {self.max_rows}")
         if out is None:
-            out = self._new(rows, width)
+            out = torch.empty_like(q) if qv[1:] == (width, rows * width) else self._new(rows, width)
             ov = (out.data_ptr(), width, rows * width)
         else:
             ov = self._view("out", out, rows, width)

@@ -220,8 +220,8 @@ class Rope:
     theta: Optional[float] = None   # set: the tables are still to be written
 
     @classmethod
-    def make(cls, seq_len, head_dim, theta, device):
-        c, s = ops.rope_table(seq_len, head_dim, theta, device=device)
+    def make(cls, seq_len, head_dim, theta, device, first=0):
+        c, s = ops.rope_table(seq_len, head_dim, theta, device=device, first=first)
         return cls(c, s, seq_len)
 
     @classmethod
@@ -268,29 +268,44 @@ def _normed(x, w, eps, M, bufs, name, rope=None):
 
 
 def decoder_layer(x, P, cfg: DecoderConfig, B, L, rope: Rope, mask="causal", prefix_len=0,
-                  bufs: Optional[Buffers] = None, qkv_out=None, mid_out=None, out=None):
+                  bufs: Optional[Buffers] = None, qkv_out=None, mid_out=None, out=None,
+                  window=None, sinks=0, cache=None):
     """One SmolLM2-style block on ``x [B*L, H]``, **in place** or into ``out``
     (``x`` is then only read); returns the fused projection buffer
     ``[B*L, q|k|v]`` whose K (post-RoPE) and V column slices are this layer's
     KV cache (vla/text_encoder_bf16.py:480-595).  ``mid_out`` (optional)
-    receives the mid-block residual (after attention)."""
+    receives the mid-block residual (after attention).
+
+    ``mask="window"``: attention within the last ``window`` rows and the first
+    ``sinks``.  ``cache`` (a :class:`~smolvla.kv_cache.KVCache`): the rows are
+    the next L tokens of every sequence (``rope`` at their positions); their K
+    and V go into it and they attend to what it holds, within its own window.
+    Both score the bf16 Q and K."""
     out = x if out is None else out
     bufs = bufs or Buffers(x.device)
     M = B * L
     qd, kvd = cfg.q_dim, cfg.kv_dim
     eps = resolve_eps(cfg.rms_eps)
     qkv = qkv_out if qkv_out is not None else bufs.get("qkv", M, qd + 2 * kvd)
+    plain = cache is not None or mask == "window"
     # remainders of the fp32 post-RoPE Q and K, which the reference module
     # scores in fp32 (vla/text_encoder_bf16.py:92-104, 117-122); the cache
     # keeps the bf16 values (:595)
-    lo = bufs.get("qkv_lo", M, qkv.stride(0))[:, :qd + 2 * kvd]
+    lo = None if plain else bufs.get("qkv_lo", M, qkv.stride(0))[:, :qd + 2 * kvd]
     a, nrm = _normed(x, P["n1"], eps, M, bufs, "xn", rope)
     ops.linear_rope(a, P["wqkv"], qd + kvd, L, rope.cos, rope.sin, out=qkv, norm=nrm, out_lo=lo)
-    q3, l3 = qkv.view(B, L, -1), lo.view(B, L, -1)
+    q3 = qkv.view(B, L, -1)
+    q, k, v = q3[:, :, :qd], q3[:, :, qd:qd + kvd], q3[:, :, qd + kvd:]
     attn = bufs.get("attn", M, qd)
-    ops.attention(q3[:, :, :qd], q3[:, :, qd:qd + kvd], q3[:, :, qd + kvd:],
-                  attn.view(B, L, qd), cfg.n_q_heads, cfg.n_kv_heads, mask, prefix_len,
-                  q_lo=l3[:, :, :qd], k_lo=l3[:, :, qd:qd + kvd])
+    if cache is not None:
+        cache.step(q, k, v, cfg.n_q_heads, out=attn.view(B, L, qd))
+    elif plain:
+        ops.attention(q, k, v, attn.view(B, L, qd), cfg.n_q_heads, cfg.n_kv_heads, mask,
+                      window=window, sinks=sinks)
+    else:
+        l3 = lo.view(B, L, -1)
+        ops.attention(q, k, v, attn.view(B, L, qd), cfg.n_q_heads, cfg.n_kv_heads, mask,
+                      prefix_len, q_lo=l3[:, :, :qd], k_lo=l3[:, :, qd:qd + kvd])
     ops.linear(attn, P["wo"], res=x, out=out)
     if mid_out is not None:
         mid_out.copy_(out)

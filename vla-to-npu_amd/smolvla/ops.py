@@ -477,10 +477,15 @@ def rope(x, heads, cos_t, sin_t, pos_offset=0, out=None, out_f32=None):
     return out
 
 
-def rope_table(max_pos, head_dim, theta, device=None):
+def rope_table(max_pos, head_dim, theta, device=None, first=0):
+    """cos and sin ``[max_pos, D/2]`` of the positions from ``first`` on."""
     dev = device or torch.device("cuda")
     c = torch.empty(max_pos, head_dim // 2, dtype=F32, device=dev)
     s = torch.empty_like(c)
+    if first:
+        _lib.call("svla_rope_table_at", _ptr(c), _ptr(s), int(first), max_pos, head_dim,
+                  float(theta), _stream())
+        return c, s
     _lib.call("svla_rope_table", _ptr(c), _ptr(s), max_pos, head_dim, float(theta), _stream())
     return c, s
 
