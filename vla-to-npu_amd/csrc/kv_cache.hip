@@ -18,10 +18,12 @@
 //     token half s >> 4 and depth half ks the codes of d = 32 ks + 8 g + 0..7;
 //     4 bits: one dword [half][ks] of the lane's 16 bytes; 8 bits: two dwords
 //     at [half] kilobyte, [ks] half of the lane's 16 bytes.
-//   V (A operand of O^T = V^T . P^T): lane (g, d & 15) holds for td = d >> 4
-//     the codes of the tokens 4 g + 0..3 and 16 + 4 g + 0..3 (the order in
-//     which S^T's accumulators become the operand P^T); 4 bits: dword [td];
-//     8 bits: [td >> 1] kilobyte, [td & 1] half.
+//   V (A operand of O^T = V^T . P^T): lane (g, d & 15) holds, for depth blocks
+//     blk = d >> 5 and token halves, the codes of the tokens 16 half + 4 g + 0..3
+//     (the order in which S^T's accumulators become the operand P^T), depths d
+//     and d + 16 of a token side by side: they share a scale, so one conversion
+//     gives both.  4 bits: a dword [blk][half], a byte a token; 8 bits: [blk]
+//     kilobyte, two dwords [half] of the lane's 16 bytes, 2 bytes a token.
 //   K scales: byte [s & 15][half][ks]; V scales: byte [g][d >> 5][8 tokens].
 // 4 bits: 1024 + 1024 + 64 + 64 bytes; 8 bits: 2048 + 2048 + 64 + 64.
 //
@@ -38,6 +40,7 @@ namespace {
 constexpr int TOK = 32;                 // tokens of a record
 constexpr int kMaxPos = 1 << 30;        // positions stay below it
 constexpr int kLost = 0x7fffffff;
+constexpr int kCUs = 256;
 constexpr int kMaxSplits = 256;
 constexpr unsigned kMaxArrivals = 64;
 
@@ -165,9 +168,8 @@ __device__ __forceinline__ unsigned block_top(u32x4 x) {
 
 // One wave builds one record in LDS and stores it whole.  Lane l takes rows
 // 8 i + l / 8, i = 0..3, and the 8 values of chunk l % 8: their codes are one
-// dword (two) of the K operand; the V operand has tokens side by side, so its
-// codes are scattered as bytes, those of a token pair put together by the pair
-// of lanes l, l ^ 8 at 4 bits.  A record that keeps older tokens is read first.
+// dword (two) of the K operand; the V operand's are scattered as bytes, put
+// together by the lanes of depths d and d + 16 at 4 bits.  A record that keeps older tokens is read first.
 //
 // The last workgroup of a sequence to have read its state stores the new one;
 // with more than kMaxArrivals of them advance_kernel does, since the arrivals at
@@ -226,31 +228,25 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
         const int g = s16 >> 2, j = half * 4 + (s & 3);
         if constexpr (BITS == 4) {
           if (in[i]) *(unsigned*)(rec + kl * 16 + (half * 2 + ks) * 4) = kc[0];
-          // the pair of tokens (s & ~1, s | 1) shares a byte: the even lane
-          // stores those of d = 8 ch + 0..3, the odd one of 8 ch + 4..7
-          const unsigned oc = __shfl_xor(vc[0], 8);
-          const bool oin = __shfl_xor((int)in[i], 8);
-          const bool odd = s & 1;
-          const unsigned lo4 = odd ? oc : vc[0], hi4 = odd ? vc[0] : oc;
-          const bool lin = odd ? oin : in[i], hin = odd ? in[i] : oin;
-          const unsigned mask = (lin ? 0x0fu : 0u) | (hin ? 0xf0u : 0u);
-          if (mask) {
+          // depths d and d + 16 share a byte: the lanes of either (ch, ch ^ 2)
+          // store half of the 8 bytes
+          const unsigned oc = __shfl_xor(vc[0], 2);
+          const bool up = ch & 2;
+          const unsigned lo4 = up ? oc : vc[0], hi4 = up ? vc[0] : oc;
+          if (in[i]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int d8 = (odd ? 4 : 0) + e, d = ch * 8 + d8;
-              uint8_t* p = rec + PART + (g * 16 + (d & 15)) * 16 + (d >> 4) * 4 + (j >> 1);
-              const unsigned w = ((lo4 >> (4 * d8)) & 15u) | (((hi4 >> (4 * d8)) & 15u) << 4);
-              *p = (uint8_t)((*p & ~mask) | (w & mask));
+              const int d8 = (up ? 4 : 0) + e;
+              rec[PART + (g * 16 + (ch & 1) * 8 + d8) * 16 + (ks * 2 + half) * 4 + (s & 3)] =
+                  (uint8_t)(((lo4 >> (4 * d8)) & 15u) | (((hi4 >> (4 * d8)) & 15u) << 4));
             }
           }
         } else if (in[i]) {
           *(u32x2*)(rec + half * 1024 + kl * 16 + ks * 8) = kc;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int d = ch * 8 + e, td = d >> 4;
-            rec[PART + (td >> 1) * 1024 + (g * 16 + (d & 15)) * 16 + (td & 1) * 8 + j] =
+          for (int e = 0; e < 8; ++e)
+            rec[PART + ks * 1024 + (g * 16 + (ch & 1) * 8 + e) * 16 + half * 8 + (s & 3) * 2 + ((ch >> 1) & 1)] =
                 (uint8_t)(vc[e >> 2] >> (8 * (e & 3)));
-          }
         }
         if (in[i] && (ch & 3) == 0) {
           rec[2 * PART + s16 * 4 + half * 2 + ks] = (uint8_t)kb;
@@ -309,17 +305,6 @@ template <int BITS> __device__ __forceinline__ bf16x8 decode8(u32x2 w, float sc)
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// 8 codes, the scale of each a byte of s0 (codes 0..3) and s1 (4..7): a pair is
-// converted with either scale and put together from the two halves
-template <int BITS> __device__ __forceinline__ bf16x8 decode8_each(u32x2 w, unsigned s0, unsigned s1) {
-  auto mix = [](unsigned lo, unsigned hi) { return (lo & 0xffffu) | (hi & 0xffff0000u); };
-  const u32x4 r = {mix(decode2<BITS, 0>(w, scale_of<0>(s0)), decode2<BITS, 0>(w, scale_of<1>(s0))),
-                   mix(decode2<BITS, 1>(w, scale_of<2>(s0)), decode2<BITS, 1>(w, scale_of<3>(s0))),
-                   mix(decode2<BITS, 2>(w, scale_of<0>(s1)), decode2<BITS, 2>(w, scale_of<1>(s1))),
-                   mix(decode2<BITS, 3>(w, scale_of<2>(s1)), decode2<BITS, 3>(w, scale_of<3>(s1)))};
-  return __builtin_bit_cast(bf16x8, r);
-}
-
 // A record in a wave's registers.
 template <int BITS> struct Rec {
   u32x4 k[BITS / 4], v[BITS / 4];
@@ -338,10 +323,6 @@ template <int BITS> struct Rec {
   __device__ __forceinline__ u32x2 kw(int half, int s) const {
     return BITS == 4 ? u32x2{k[0][half * 2 + s], 0u}
                      : u32x2{k[BITS == 4 ? 0 : half][s * 2], k[BITS == 4 ? 0 : half][s * 2 + 1]};
-  }
-  __device__ __forceinline__ u32x2 vw(int td) const {
-    return BITS == 4 ? u32x2{v[0][td], 0u}
-                     : u32x2{v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2], v[BITS == 4 ? 0 : td >> 1][(td & 1) * 2 + 1]};
   }
   __device__ __forceinline__ void store(uint8_t* p, int lane) const {
     constexpr int PART = kPart<BITS>;
@@ -389,7 +370,6 @@ template <int BITS> struct Rec {
         put(ks, byte, 8 * (half * 2 + s), 255u);
       }
     }
-    const int j = half * 4 + (slot & 3);
     const unsigned short* vb = reinterpret_cast<const unsigned short*>(vn);
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
@@ -401,26 +381,23 @@ template <int BITS> struct Rec {
       const u32x2 code = encode8<BITS>(x, byte);
       if (grp == (s16 >> 2)) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if constexpr (BITS == 4) {
-            unsigned y = v[0][2 * blk + w];
-            put(y, code[0] >> (4 * w), 4 * j, 15u);
-            v[0][2 * blk + w] = y;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              if (q == half) {
-                unsigned y = v[blk][2 * w + q];
-                put(y, code[0] >> (8 * w), 8 * (j & 3), 255u);
-                v[blk][2 * w + q] = y;
-              }
-          }
-        }
-#pragma unroll
         for (int q = 0; q < 2; ++q)
           if (q == half) {
+            if constexpr (BITS == 4) {
+              unsigned y = v[0][blk * 2 + q];
+              put(y, code[0], 8 * (slot & 3), 255u);
+              v[0][blk * 2 + q] = y;
+            } else {
+#pragma unroll
+              for (int w = 0; w < 2; ++w)
+                if (w == ((slot >> 1) & 1)) {
+                  unsigned y = v[blk][q * 2 + w];
+                  put(y, code[0], 16 * (slot & 1), 0xffffu);
+                  v[blk][q * 2 + w] = y;
+                }
+            }
             unsigned y = vs[blk * 2 + q];
-            put(y, byte, 8 * (j & 3), 255u);
+            put(y, byte, 8 * (slot & 3), 255u);
             vs[blk * 2 + q] = y;
           }
       }
@@ -429,8 +406,28 @@ template <int BITS> struct Rec {
   template <int HALF, int S> __device__ __forceinline__ bf16x8 kfrag() const {
     return decode8<BITS>(kw(HALF, S), scale_of<HALF * 2 + S>(ks));
   }
-  __device__ __forceinline__ bf16x8 vfrag(int td) const {
-    return decode8_each<BITS>(vw(td), vs[(td >> 1) * 2], vs[(td >> 1) * 2 + 1]);
+  // the operands of depths 32 blk + 0..15 and + 16..31: a conversion per token,
+  // then the halves of two tokens are sorted out
+  template <int BLK> __device__ __forceinline__ void vfrags(bf16x8& lo, bf16x8& hi) const {
+    unsigned t[8];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const u32x2 w = BITS == 4 ? u32x2{v[0][BLK * 2 + hf], 0u}
+                                : u32x2{v[BITS == 4 ? 0 : BLK][hf * 2], v[BITS == 4 ? 0 : BLK][hf * 2 + 1]};
+      const unsigned sc = vs[BLK * 2 + hf];
+      t[hf * 4 + 0] = decode2<BITS, 0>(w, scale_of<0>(sc));
+      t[hf * 4 + 1] = decode2<BITS, 1>(w, scale_of<1>(sc));
+      t[hf * 4 + 2] = decode2<BITS, 2>(w, scale_of<2>(sc));
+      t[hf * 4 + 3] = decode2<BITS, 3>(w, scale_of<3>(sc));
+    }
+    u32x4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x05040100u);
+      b[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x07060302u);
+    }
+    lo = __builtin_bit_cast(bf16x8, a);
+    hi = __builtin_bit_cast(bf16x8, b);
   }
 };
 
@@ -483,12 +480,13 @@ __global__ __launch_bounds__(64) void read_kernel(ReadArgs a) {
     put_k(0, 1, r.template kfrag<0, 1>());
     put_k(1, 0, r.template kfrag<1, 0>());
     put_k(1, 1, r.template kfrag<1, 1>());
+    bf16x8 vf[4];
+    r.template vfrags<0>(vf[0], vf[1]);
+    r.template vfrags<1>(vf[2], vf[3]);
 #pragma unroll
-    for (int td = 0; td < 4; ++td) {
-      const bf16x8 x = r.vfrag(td);
+    for (int td = 0; td < 4; ++td)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sv[((j >> 2) * 16 + 4 * grp + (j & 3)) * LD + td * 16 + col] = x[j];
-    }
+      for (int j = 0; j < 8; ++j) sv[((j >> 2) * 16 + 4 * grp + (j & 3)) * LD + td * 16 + col] = vf[td][j];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -738,12 +736,18 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
           pf[t][i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t])));
         o[t][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], o[t][4], 0, 0, 0);
       }
+      bf16x8 va, vb;
+      r.template vfrags<0>(va, vb);
 #pragma unroll
-      for (int td = 0; td < 4; ++td) {
-        const bf16x8 vf = r.vfrag(td);
+      for (int t = 0; t < QT; ++t) {
+        o[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[t], o[t][0], 0, 0, 0);
+        o[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pf[t], o[t][1], 0, 0, 0);
+      }
+      r.template vfrags<1>(va, vb);
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-          o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[t][td], 0, 0, 0);
+      for (int t = 0; t < QT; ++t) {
+        o[t][2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[t], o[t][2], 0, 0, 0);
+        o[t][3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pf[t], o[t][3], 0, 0, 0);
       }
     };
     // the newest record, where the new row goes: its wave takes it first
@@ -926,8 +930,9 @@ Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   // records of a sequence, at most; a wave should have 4 of them
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
   const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
-  const long want = 1024 / p.qt;
-  p.splits = (int)max(1L, min(min((want + x * bh - 1) / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
+  // workgroups that are resident at once (registers): one round of them
+  const long room = kCUs * (p.qt == 4 ? 2 : 3);
+  p.splits = (int)max(1L, min(min(room / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
   p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
   return p;
 }
