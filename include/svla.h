@@ -537,7 +537,8 @@ int svla_f32_to_bf16(const float* x, void* y, long n, svla_stream_t stream);
  * position that are > position - window or < sinks, and < lens[b] (device
  * int32 per sequence, clamped to [0, sk]; NULL: sk).  A row that sees nothing
  * gives zeros, and no key that a row does not see reaches it, be it infinite
- * or NaN.  window >= 1, sinks >= 0, q_pos >= 0, scale > 0. */
+ * or NaN.  window >= 1, sinks >= 0, q_pos >= 0, scale > 0; ldk, ldv <= 2^24.
+ * o may be q. */
 int svla_attention_window_bf16(const void* q, int ldq, long q_bs, const void* k, int ldk, long k_bs,
                                const void* v, int ldv, long v_bs, void* o, int ldo, long o_bs,
                                int batch, int sq, int sk, int hq, int hkv, int head_dim,
@@ -604,7 +605,7 @@ int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void*
  * KV head h * n_kv_heads / hq.  Scores, statistics and sums fp32,
  * probabilities bf16, bf16 out.  Rows behind counts[b] are written as zeros.  A
  * sequence of which a position that the call needs has left the ring (or that
- * is lost, or holds fewer tokens than counts[b]) gives NaN.  scale > 0,
+ * is lost, or holds fewer tokens than counts[b]) gives NaN.  scale > 0, o may be q,
  * rows * hq <= 2^24.  scratch: svla_kv_attention_scratch bytes, 16-byte aligned,
  * of this call alone until it is done (NULL where that is 0). */
 long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window);

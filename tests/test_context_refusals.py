@@ -97,7 +97,7 @@ def test_bad_window_arguments():
         q, ldq, qbs, k, ldk, 0, v, 64, 0, o, ldo, 0, batch, sq, sk, hq, hkv, d, scale, q_pos, None,
         window, sinks, None)
     for kw in (dict(q=None), dict(k=ODD), dict(o=None), dict(ldq=64), dict(ldk=60), dict(ldo=130),
-               dict(qbs=4), dict(batch=-1), dict(batch=65536), dict(sq=-1), dict(sk=0), dict(hq=0),
+               dict(qbs=4), dict(ldk=2 ** 24 + 64), dict(batch=-1), dict(batch=65536), dict(sq=-1), dict(sk=0), dict(hq=0),
                dict(hq=3, hkv=2), dict(d=32), dict(scale=0.0), dict(scale=float("inf")),
                dict(q_pos=-1), dict(q_pos=2 ** 30), dict(window=0), dict(sinks=-1)):
         assert call(**kw) == -22, kw
@@ -106,7 +106,9 @@ def test_bad_window_arguments():
 
 @pytest.mark.parametrize("kw", [dict(fmt="fp4"), dict(batch=0), dict(n_kv_heads=0), dict(rows=0),
                                 dict(window=0), dict(max_len=None), dict(max_len=0), dict(sinks=2),
-                                dict(window=4, sinks=-1), dict(device="cpu")])
+                                dict(window=4, sinks=-1), dict(device="cpu"), dict(max_len=2 ** 32 + 5),
+                                dict(batch=2 ** 32 + 1), dict(window=2 ** 32 + 1, max_len=None),
+                                dict(window=4, sinks=2 ** 32)])
 def test_constructor(kw):
     from smolvla.kv_cache import KVCache
     args = dict(batch=1, n_kv_heads=1, max_len=32)

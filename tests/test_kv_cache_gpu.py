@@ -278,6 +278,87 @@ def test_a_long_stream_through_the_ring(fmt):
     cache.check()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hq,hkv", [(3, 3), (16, 1), (40, 2), (64, 1), (96, 1)])
+@pytest.mark.parametrize("held", [0, 31, 32, 1100])
+def test_a_step_of_one_token(fmt, hq, hkv, held):
+    """One new row per sequence (of some): written by the attention itself where
+    one workgroup has all of a record's columns; the cache is then the one that
+    append leaves."""
+    g = gen(held + hq)
+    cache = KVCache(3, hkv, fmt=fmt, max_len=held + 3)
+    other = KVCache(3, hkv, fmt=fmt, max_len=held + 3)
+    want = ref.CacheRef(3, hkv, fmt)
+    k, v = rand(g, 3, held, hkv * 64), rand(g, 3, held, hkv * 64)
+    for c in (cache, other, want):
+        c.append(k, v)
+    for counts in (None, ints(1, 0, 1), None):
+        q, k, v = rand(g, 3, 1, hq * 64), rand(g, 3, 1, hkv * 64), rand(g, 3, 1, hkv * 64)
+        got = cache.step(q, k, v, hq, counts=counts)
+        other.append(k, v, counts=counts)
+        want.append(k, v, counts)
+        close(got, want.attend(q, hq, counts))
+    assert torch.equal(cache.state, other.state)
+    for x, y in zip(cache.read(), other.read()):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_a_step_at_a_position(fmt):
+    """Steps that go back, one that skips ahead (lost), and one whose row is NaN."""
+    g = gen(20)
+    cache, want = KVCache(3, 2, max_len=100, fmt=fmt), ref.CacheRef(3, 2, fmt)
+    k, v = rand(g, 3, 70, 128), rand(g, 3, 70, 128)
+    cache.append(k, v)
+    want.append(k, v)
+    q, k, v = rand(g, 3, 1, 384), rand(g, 3, 1, 128), rand(g, 3, 1, 128)
+    v[2, 0, 40] = float("nan")
+    at = ints(70, 33, 64)
+    got = cache.step(q, k, v, 6, at=at)
+    want.append(k, v, at=at)
+    close(got, want.attend(q, 6))
+    same(cache.read(at, 1)[1], torch.stack([x[-1:] for x in want.v]))
+    got = cache.step(q, k, v, 6, at=ints(72, 0, 1))
+    want.append(k, v, at=[0, 0, 1])
+    assert torch.isnan(got[0]).all() and not torch.isnan(got[1]).any()
+    close(got[1:], tuple(x[1:] for x in want.attend(q, 6)))
+    with pytest.raises(RuntimeError, match=r"\[0\] were written"):
+        cache.check()
+
+
+def test_a_first_score_far_below_the_others():
+    """Scores that outgrow the first record's by hundreds of powers of two."""
+    g = gen(21)
+    for rows in (1, 20):
+        cache, want = KVCache(1, 1, max_len=900, fmt="mxfp8"), ref.CacheRef(1, 1, "mxfp8")
+        k, v = rand(g, 1, 900, 64), rand(g, 1, 900, 64)
+        k *= torch.linspace(0.01, 60, 900, device="cuda")[:, None].to(BF16)
+        v[0, 100:200] *= 2.0 ** 104
+        cache.append(k, v)
+        want.append(k, v)
+        q = rand(g, 1, rows, 128, scale=2.0)
+        close(cache.attend(q, 2, scale=2.0), want.attend(q, 2, scale=2.0))
+
+
+def test_time_before_batch_and_in_place():
+    """[T, B, .] tensors as [B, T, .] views, and the output over the queries."""
+    g = gen(22)
+    cache, want = KVCache(3, 1, max_len=60), ref.CacheRef(3, 1, "mxfp4")
+    q, k, v = (rand(g, 50, 3, w).transpose(0, 1) for w in (128, 64, 64))
+    expect = q.clone()
+    out = torch.empty(50, 3, 128, dtype=BF16, device="cuda").transpose(0, 1)
+    cache.step(q, k, v, 2, out=out)
+    want.append(k, v)
+    close(out, want.attend(expect, 2))
+    cache.attend(q, 2, out=q)
+    assert torch.equal(q, out)
+    ko, vo = (torch.empty(60, 3, 64, dtype=BF16, device="cuda").transpose(0, 1) for _ in range(2))
+    cache.read(0, 60, k_out=ko, v_out=vo)
+    same(ko[:, :50], ref.stored(k.cpu(), "mxfp4"))
+    same(vo[:, :50], ref.stored(v.cpu(), "mxfp4"))
+    assert (ko[:, 50:] == 0).all()
+
+
 # ------------------------------------------------------------------- errors ---
 @pytest.mark.parametrize("fmt", FMTS)
 def test_lost_sequences(fmt):
@@ -434,8 +515,13 @@ def test_refusals():
         cache.step(k, rand(g, 2, 2, 128), rand(g, 2, 2, 128), 2)
     with pytest.raises(ValueError):
         cache.read()                                            # no max_len
-    with pytest.raises(ValueError):
-        cache.read(-1, 4)
+    for start in (-1, 2 ** 32):
+        with pytest.raises(ValueError):
+            cache.read(start, 4)
+    with pytest.raises(ValueError, match="overlap"):
+        cache.read(0, 4, k_out=rand(g, 1, 4, 128).expand(2, -1, -1))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.attend(k, 2, out=k[:1].expand(2, -1, -1))
     assert cache.lengths.tolist() == [0, 0]
     # nothing to do
     cache.append(k[:, :0], k[:, :0])

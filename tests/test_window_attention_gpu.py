@@ -150,6 +150,26 @@ def test_a_window_over_everything_equals_the_causal_kernel():
         assert (a.float() - w.float()).abs().max() <= scale
 
 
+def test_sizes_past_32_bits_mean_everything():
+    g = gen(11)
+    q, k, v = rand(g, 1, 90, 128), rand(g, 1, 90, 64), rand(g, 1, 90, 64)
+    a = ops.attention(q, k, v, torch.empty_like(q), 2, 1, mask="window", window=90)
+    for kw in (dict(window=2 ** 32 + 1), dict(window=1, sinks=2 ** 32 + 1)):
+        b = ops.attention(q, k, v, torch.empty_like(q), 2, 1, mask="window", **kw)
+        assert torch.equal(a, b)
+
+
+def test_time_before_batch_and_in_place():
+    """[T, B, .] tensors as [B, T, .] views, and the output over the queries."""
+    g = gen(12)
+    q, k, v = (rand(g, 70, 3, w).transpose(0, 1) for w in (128, 64, 64))
+    out = torch.empty(70, 3, 128, dtype=BF16, device="cuda").transpose(0, 1)
+    check(q, k, v, 2, 1, 20, 2, out=out)
+    want = out.clone()
+    ops.attention(q, k, v, q, 2, 1, mask="window", window=20, sinks=2)
+    assert torch.equal(q, want)
+
+
 def test_captured_call():
     g = gen(8)
     q, k, v = rand(g, 2, 100, 128), rand(g, 2, 100, 64), rand(g, 2, 100, 64)
@@ -179,11 +199,11 @@ def test_refusals():
     for kw in (dict(window=None), dict(q=q.float()), dict(k=k[:1]), dict(v=k[:, :4]),
                dict(o=o[:, :, :64]), dict(lens=torch.ones(1, dtype=torch.int32, device="cuda")),
                dict(lens=torch.ones(2, device="cuda")), dict(prefix_len=3), dict(q_lo=q),
-               dict(mask="causal"), dict(q=q.cpu()), dict(mask="none", window=None, sinks=1)):
+               dict(window=0), dict(window=-1), dict(sinks=-1), dict(q_pos=-1), dict(q_pos=2 ** 32),
+               dict(o=o[:1].expand(2, -1, -1)), dict(mask="causal"), dict(q=q.cpu()), dict(mask="none", window=None, sinks=1)):
         with pytest.raises(ValueError):
             call(**kw)
-    for kw in (dict(window=0), dict(window=-1), dict(sinks=-1), dict(q_pos=-1), dict(scale=0.0),
-               dict(scale=float("nan")), dict(hq=2, hkv=3, k=rand(g, 2, 8, 192), v=rand(g, 2, 8, 192)),
+    for kw in (dict(scale=0.0), dict(scale=float("nan")), dict(hq=2, hkv=3, k=rand(g, 2, 8, 192), v=rand(g, 2, 8, 192)),
                dict(q=rand(g, 2, 8, 129)[:, :, 1:])):
         with pytest.raises(SvlaError):
             call(**kw)

@@ -29,6 +29,7 @@ BF16 = torch.bfloat16
 HEAD_DIM = 64
 SCALE = 1.0 / math.sqrt(HEAD_DIM)
 TOKENS = 32                     # tokens of a record
+MAX_POS = 1 << 30               # positions stay below it
 FORMATS = {"mxfp4": 4, "mxfp8": 8}
 
 
@@ -80,6 +81,8 @@ class KVCache:
         self.max_rows = rows if max_len is None else None
         self.max_len = max_len
         self.ring = (ring + TOKENS - 1) // TOKENS * TOKENS
+        if self.ring > MAX_POS or sinks > MAX_POS // 2 or batch * n_kv_heads > 65535:
+            raise ValueError("KVCache: size not supported")
         self._lib = _lib.load()
         nbytes = self._lib.svla_kv_cache_bytes(batch, n_kv_heads, HEAD_DIM, FORMATS[fmt], sinks,
                                                self.ring)
@@ -116,7 +119,7 @@ class KVCache:
                 raise RuntimeError(f"KVCache: sequences {over} hold more than {self.max_len} tokens")
 
     # ---------------------------------------------------------------- calls --
-    def _view(self, name, t, rows, width):
+    def _view(self, name, t, rows, width, written=False):
         """(address, row stride, batch stride) of a bf16 ``[B, rows, >= width]``
         view; a stride that no index uses is any valid one."""
         try:
@@ -128,6 +131,9 @@ class KVCache:
             ok = False
         if not ok:
             raise ValueError(_bad(name, t, self.batch, rows, width, self.device))
+        if written and b > 1 and not (sb >= (r - 1) * sr + width
+                                      or sb >= width and sr >= (b - 1) * sb + width):
+            raise ValueError(f"{name}: rows must not overlap")
         return t.data_ptr(), (sr if r > 1 else (w + 7) // 8 * 8), (sb if b > 1 else 0)
 
     def _new(self, rows, width):
@@ -175,17 +181,17 @@ class KVCache:
             k_out = self._new(rows, width)
             kv = (k_out.data_ptr(), width, rows * width)
         else:
-            kv = self._view("k_out", k_out, rows, width)
+            kv = self._view("k_out", k_out, rows, width, True)
         if v_out is None:
             v_out = self._new(rows, width)
             kv += (v_out.data_ptr(), width, rows * width)
         else:
-            kv += self._view("v_out", v_out, rows, width)
+            kv += self._view("v_out", v_out, rows, width, True)
         starts = None
         if torch.is_tensor(start):
             starts, start = self._ints("start", start), 0
-        elif start < 0:
-            raise ValueError(f"start must not be negative, got {start}")
+        elif not 0 <= start <= MAX_POS:
+            raise ValueError(f"start must be a position, got {start}")
         self._call("svla_kv_read_bf16", *kv, start, starts, rows)
         return k_out, v_out
 
@@ -216,7 +222,7 @@ class KVCache:
             out = torch.empty_like(q) if qv[1:] == (width, rows * width) else self._new(rows, width)
             ov = (out.data_ptr(), width, rows * width)
         else:
-            ov = self._view("out", out, rows, width)
+            ov = self._view("out", out, rows, width, True)
         key = (rows, n_heads)
         nbytes = self._scratch.get(key)
         if nbytes is None:

@@ -370,6 +370,8 @@ def _attention_window(q, k, v, out, hq, hkv, scale, window, sinks, lens, q_pos):
         raise ValueError('attention: mask="window" needs window')
     if not q.is_cuda:
         raise ValueError("smolvla ops take GPU tensors (no CPU fallback)")
+    if not (window >= 1 and sinks >= 0 and 0 <= q_pos < 1 << 30):
+        raise ValueError(f"attention: window {window}, sinks {sinks} or q_pos {q_pos} out of range")
     args = []
     for t, rows, heads in ((q, Sq, hq), (k, Sk, hkv), (v, Sk, hkv), (out, Sq, hq)):
         b, r, w = t.shape
@@ -379,11 +381,15 @@ def _attention_window(q, k, v, out, hq, hkv, scale, window, sinks, lens, q_pos):
         # (a stride that no index uses need not be a valid one)
         sb, sr, _ = t.stride()
         args += [t.data_ptr(), sr if r > 1 else (w + 7) // 8 * 8, sb if b > 1 else 0]
+    width = hq * 64
+    if B > 1 and not (sb >= (r - 1) * sr + width or sb >= width and sr >= (B - 1) * sb + width):
+        raise ValueError("attention: rows of out must not overlap")
     if lens is not None and (lens.dtype is not torch.int32 or lens.shape != (B,)
                              or not lens.is_contiguous() or lens.device != device):
         raise ValueError(f"attention: lens must be contiguous int32 [{B}] on {device}")
     args += [B, Sq, Sk, hq, hkv, 64, float(scale), int(q_pos),
-             None if lens is None else lens.data_ptr(), int(window), int(sinks)]
+             None if lens is None else lens.data_ptr(), min(int(window), 1 << 30),
+             min(int(sinks), 1 << 30)]
     if torch.cuda.current_device() == device.index:
         _lib.call("svla_attention_window_bf16", *args,
                   torch._C._cuda_getCurrentRawStream(device.index))
