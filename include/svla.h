@@ -606,7 +606,7 @@ int svla_kv_read_bf16(const svla_kv_cache* c, void* k, int ldk, long k_bs, void*
  * probabilities bf16, bf16 out.  Rows behind counts[b] are written as zeros.  A
  * sequence of which a position that the call needs has left the ring (or that
  * is lost, or holds fewer tokens than counts[b]) gives NaN.  scale > 0, o may be q,
- * rows * hq <= 2^24.  scratch: svla_kv_attention_scratch bytes, 16-byte aligned,
+ * rows * hq <= 2^24, hq <= 255 n_kv_heads.  scratch: svla_kv_attention_scratch bytes, 16-byte aligned,
  * of this call alone until it is done (NULL where that is 0). */
 long svla_kv_attention_scratch(const svla_kv_cache* c, int rows, int hq, int window);
 int svla_kv_attention_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void* o,

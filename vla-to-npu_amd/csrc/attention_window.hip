@@ -129,21 +129,20 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
   f32x4 o[QT][5];
   float m_run[QT], m_off[QT];
   const float c = p.scale_log2;
-  auto clear = [&]() {
+  auto clear = [&](float m) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
       for (int t = 0; t < 5; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m_run[qt] = -INFINITY;
+      m_run[qt] = m;
       m_off[qt] = 0.f;
     }
   };
-  clear();
+  clear(0.f);
   bf16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.0f);
-  int track = 0;           // follow the maximum in every block
-  bool started = false;    // every row of the wave has seen a key
+  int track = 0;           // the second time over the keys
 
   // Byte offsets of the lane's operand reads within a stage (kv_off: a key's row
   // is 128 bytes, its 16-byte chunks are swapped by the key's low bits, which
@@ -203,7 +202,6 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
   // Follows the maximum, which moves only when a score passes it by 2^8 as in
   // attention_kernel.
   auto follow = [&]() __attribute__((always_inline)) {
-    bool seen_all = true;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       float mx = sacc[0][qt][0];
@@ -219,9 +217,7 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
         m_run[qt] = m_new;
         m_off[qt] = -((m_new == -INFINITY ? 0.f : m_new) * c);
       }
-      seen_all = seen_all && m_run[qt] != -INFINITY;
     }
-    started = __builtin_amdgcn_ballot_w64(!seen_all) == 0;
   };
   // Takes infinities and NaNs out of V; returns whether there were any.
   auto take_out = [&]() __attribute__((always_inline)) {
@@ -291,11 +287,13 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
   };
-  // Only the first keys set the maximum: any reference gives the same quotient
-  // as long as nothing overflows.  Where something does (scores over 2^100 times
-  // the first ones, V that large, infinite or NaN: also behind the mask, as
-  // 0 * NaN), the workgroup goes over its keys once more, following the maximum,
-  // and a row then meets only what it sees, infinities and NaNs apart.
+  // Softmax needs no maximum where exp(s) itself neither over- nor underflows:
+  // any reference gives the same quotient, and bf16 keeps fp32's range.  So the
+  // first time over the keys takes the reference 0.  Where a row's sum leaves
+  // [2^-60, 2^100], or an output 2^100 (also by infinities and NaNs, even from
+  // behind the mask, as 0 * NaN), the workgroup goes over its keys once more,
+  // following the maximum, and a row then meets only what it sees, infinities
+  // and NaNs apart.
   // The wave's blocks in the list: [see0, see1) of the windows' blocks hold keys
   // that some row sees, [full0, full1) only keys that all do; of the sinks' the
   // first sink_full.
@@ -325,8 +323,10 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
         bool odd = false;
         score(0);
         if (part) mask(k0);
-        if (track || !started) follow();
-        if (track) odd = take_out();
+        if (track) {
+          follow();
+          odd = take_out();
+        }
         accumulate();
         if (track && odd) put_back(0, k0);
         score(1);
@@ -334,8 +334,10 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
           if (!(k1 <= whi && k1 < len && (k1 + 31 > wlo - p.window || k1 < p.sinks))) goto done;
           mask(k1);
         }
-        if (track || !started) follow();
-        if (track) odd = take_out();
+        if (track) {
+          follow();
+          odd = take_out();
+        }
         accumulate();
         if (track && odd) put_back(1, k1);
       }
@@ -346,17 +348,20 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
       for (int i = 0; i < 4; ++i) vofs[i] ^= STAGE;
       sync_step();
     }
-    bool over = false;
+    bool bad = false;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
+    for (int qt = 0; qt < QT; ++qt) {
+      float top = o[qt][4][0];
 #pragma unroll
-      for (int t = 0; t < 5; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) over |= !(fabsf(o[qt][t][i]) < 0x1p100f);
-    if (track || !__syncthreads_or(over)) break;
+        for (int i = 0; i < 4; ++i) top = smax(top, fabsf(o[qt][t][i]));
+      const bool sees_some = last[qt] > max(before[qt], -1) || (p.sinks > 0 && last[qt] >= 0);
+      bad |= sees_some && !(top < 0x1p100f && o[qt][4][0] >= 0x1p-60f);
+    }
+    if (track || !__syncthreads_or(bad && qw < p.sq)) break;
     track = 1;
-    started = false;
-    clear();
+    clear(-INFINITY);
     // back to the first stage
     if (nb & 1) {
 #pragma unroll

@@ -508,6 +508,7 @@ struct AttendArgs {
   long ldo, o_bs;
   const int* counts;
   int rows, group, window;
+  unsigned group_inv;         // j / group = (j * group_inv) >> 32 for the columns j
   float scale_log2;
   int splits;
   float *part, *stat;         // [batch * heads][columns][splits] x 64 and x 2
@@ -531,6 +532,10 @@ __device__ __forceinline__ View view_of(const AttendArgs& a, int b, int n, int l
   return v;
 }
 
+__device__ __forceinline__ int row_of(const AttendArgs& a, int j) {
+  return a.group_inv ? (int)__umulhi((unsigned)j, a.group_inv) : j;
+}
+
 // Output of one column: 4 depths from d on; rows behind the count are zeros.
 __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View& v, int r) {
   const float inv = l > 0.f ? 1.0f / l : l;        // nothing visible: 0; NaN stays
@@ -552,11 +557,12 @@ __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View&
 // one column (lane & 15); the accumulators of S^T are the operand P^T as they
 // stand.  The sum of the rounded probabilities is an MFMA with a row of ones.
 //
-// Only the first tokens set the maximum: any reference gives the same quotient
-// as long as nothing overflows.  Where something does (scores over 2^100 times
-// the first ones, V that large or NaN: also behind the mask, as 0 * NaN), the
-// wave goes over its records once more, following the maximum, and a column
-// then meets only what it sees, NaN blocks apart.
+// Softmax needs no maximum where exp(s) itself neither over- nor underflows: any
+// reference gives the same quotient, and bf16 keeps fp32's range.  So the first
+// time over the records takes the reference 0.  A wave of which a column's sum
+// leaves [2^-60, 2^100], or an output 2^100 (also by infinities and NaNs, even
+// from behind the mask, as 0 * NaN), goes over its records once more, following
+// the maximum, and a column then meets only what it sees, NaN blocks apart.
 //
 // PF records are in registers or on their way to them.
 template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2) : 8 / BITS;
@@ -564,8 +570,9 @@ template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2)
 // NEW: one new row per sequence is written on the way.
 template <int BITS, int QT, bool NEW>
 __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs a) {
-  constexpr int PF = kAhead<BITS, QT>, KW = 4, LD = 16 * QT + 1;
-  __shared__ float s_part[KW][D + 2][LD];          // per wave: 64 depths, reference, sum
+  constexpr int PF = kAhead<BITS, QT>, KW = 4, LD = D + 4;
+  // per wave and column: 64 depths, reference, sum
+  __shared__ __attribute__((aligned(16))) float s_part[KW][16 * QT][LD];
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = lane >> 4, col = lane & 15;
@@ -585,29 +592,29 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int j = min(col0 + t * 16 + col, ncol - 1);
-    const int r = j / a.group, hh = h * a.group + j - r * a.group;
+    const int r = row_of(a, j), hh = h * a.group + j - r * a.group;
     qpos[t] = r < count ? first + r : -1;
     const bf16* q = a.q + b * a.q_bs + r * a.ldq + hh * D;
 #pragma unroll
     for (int s = 0; s < 2; ++s) qf[t][s] = ld8(q + s * 32 + grp * 8);
   }
   // positions of the workgroup's first and last row
-  const int r0 = col0 / a.group, r1 = (min(col0 + QT * 16, ncol) - 1) / a.group;
+  const int r0 = row_of(a, col0), r1 = row_of(a, min(col0 + QT * 16, ncol) - 1);
   const int qlo = first + min(r0, count - 1), qhi = first + min(r1, count - 1);
 
   f32x4 o[QT][5];
   float m_run[QT], m_off[QT];
   const float cs = a.scale_log2;
-  auto clear = [&]() {
+  auto clear = [&](float m) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
 #pragma unroll
       for (int i = 0; i < 5; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m_run[t] = -INFINITY;
+      m_run[t] = m;
       m_off[t] = 0.f;
     }
   };
-  clear();
+  clear(-INFINITY);
   bf16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.0f);
@@ -634,10 +641,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
       }
       return base + (long)u * kRec<BITS>;
     };
-    int track = 0;             // follow the maximum at every record
-    bool started = false;      // every column of the wave has seen a token
-    // One record.  FOLLOW: the maximum moves and, from the second time over the
-    // records on, columns meet only what they see.
+    // One record.  FOLLOW: the second time.
     auto step = [&](auto FOLLOW, Rec<BITS>& r, int ti) __attribute__((always_inline)) {
       const bool sink = ti < ns;
       const int pos0 = sink ? ti * TOK : c.sinks + (u0 + ti - ns) * TOK;
@@ -672,7 +676,6 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
       }
       if constexpr (decltype(FOLLOW)::value) {
         // the maximum moves when a score passes it by 2^8 (exp2 units)
-        bool seen_all = true;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           float mx = sc[t][0][0];
@@ -688,11 +691,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
             m_run[t] = m_new;
             m_off[t] = m_new == -INFINITY ? 0.f : -m_new * cs;
           }
-          seen_all = seen_all && (m_run[t] != -INFINITY || qpos[t] < 0);
         }
-        started = __builtin_amdgcn_ballot_w64(!seen_all) == 0;
-      }
-      if (decltype(FOLLOW)::value && track) {
         // NaN blocks (scale byte 0xff) count as 0 in V and are added to the
         // columns that see them
 #pragma unroll 1
@@ -752,62 +751,63 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
     };
     // the newest record, where the new row goes: its wave takes it first
     const bool newest = NEW && t1 == total && kw == ((total - 1 - t0) & (KW - 1));
-    const int tend = newest ? t1 - 1 : t1;
-    while (from < t1) {
-      Rec<BITS> r0, r[PF];
-      int cur = newest ? total - 1 : from, ti = newest ? from : from + KW;
-      r0.load(addr(cur), lane);
+    const int mine = from < t1 ? (t1 - 1 - from) / KW + 1 : 0;       // records of this wave
+    auto place = [&](int i) {                                        // its i-th one
+      return NEW && newest ? (i == 0 ? total - 1 : from + (i - 1) * KW) : from + i * KW;
+    };
+    auto insert = [&](Rec<BITS>& r) {
+      const int slot = (span.p0 < c.sinks ? span.p0 : span.p0 - c.sinks) & (TOK - 1);
+      r.insert(a.k + b * a.k_bs + h * D, a.v + b * a.v_bs + h * D, slot, lane);
+    };
+    if (mine > 0) {
+      Rec<BITS> r[PF];
 #pragma unroll
-      for (int i = 0; i < PF; ++i) r[i].load(addr(ti + i * KW), lane);
-      if (newest) {
-        const int slot = (span.p0 < c.sinks ? span.p0 : span.p0 - c.sinks) & (TOK - 1);
-        r0.insert(a.k + b * a.k_bs + h * D, a.v + b * a.v_bs + h * D, slot, lane);
-        r0.store(const_cast<uint8_t*>(addr(cur)), lane);
+      for (int i = 0; i < PF; ++i) r[i].load(addr(place(i)), lane);
+      if (NEW && newest) {
+        insert(r[0]);
+        r[0].store(const_cast<uint8_t*>(addr(total - 1)), lane);
       }
-      bool more = false;
-      for (;;) {
-        step(std::true_type{}, r0, cur);
-        if (ti >= tend || !(track || !started)) break;
-        cur = ti;
-        ti += KW;
-        r0.load(addr(cur), lane);
-        more = true;
-      }
-      if (more && ti < tend) {
-#pragma unroll
-        for (int i = 0; i < PF; ++i) r[i].load(addr(ti + i * KW), lane);
-      }
-      for (; ti < tend; ti += PF * KW) {
+      for (int at = 0; at < mine; at += PF) {
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-          if (ti + i * KW >= tend) break;
-          step(std::false_type{}, r[i], ti + i * KW);
-          r[i].load(addr(ti + (i + PF) * KW), lane);
+          if (at + i >= mine) break;
+          step(std::false_type{}, r[i], place(at + i));
+          r[i].load(addr(place(at + i + PF)), lane);
         }
       }
-      bool over = false;
+      bool bad = false;
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+      for (int t = 0; t < QT; ++t) {
+        float top = o[t][4][0];
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) over |= !(fabsf(o[t][i][e]) < 0x1p100f);
-      if (track || !__builtin_amdgcn_ballot_w64(over)) break;
-      track = 1;
-      clear();
+          for (int e = 0; e < 4; ++e) top = smax(top, fabsf(o[t][i][e]));
+        bad |= qpos[t] >= 0 && !(top < 0x1p100f && o[t][4][0] >= 0x1p-60f);
+        m_run[t] = 0.f;
+      }
+      if (__builtin_amdgcn_ballot_w64(bad)) {
+        clear(-INFINITY);
+#pragma unroll 1
+        for (int at = 0; at < mine; ++at) {
+          Rec<BITS> x;
+          x.load(addr(place(at)), lane);
+          if (NEW && newest && at == 0) insert(x);
+          step(std::true_type{}, x, place(at));
+        }
+      }
     }
   }
 
   // join the waves: the 4 QT tiles (16 columns x 16 depths) are shared out
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
+    float* part = s_part[kw][t * 16 + col];
 #pragma unroll
-    for (int td = 0; td < 4; ++td)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s_part[kw][td * 16 + grp * 4 + i][t * 16 + col] = o[t][td][i];
+    for (int td = 0; td < 4; ++td) *(f32x4*)(part + td * 16 + grp * 4) = o[t][td];
     if (grp == 0) {
-      s_part[kw][D][t * 16 + col] = m_run[t];
-      s_part[kw][D + 1][t * 16 + col] = o[t][4][0];
+      part[D] = m_run[t];
+      part[D + 1] = o[t][4][0];
     }
   }
   __syncthreads();
@@ -824,26 +824,24 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
   float mw[KW], m = -INFINITY;
 #pragma unroll
   for (int w = 0; w < KW; ++w) {
-    mw[w] = s_part[w][D][jj];
+    mw[w] = s_part[w][jj][D];
     m = smax(m, mw[w]);
   }
   float l = 0.f;
 #pragma unroll
   for (int w = 0; w < KW; ++w) {
     mw[w] = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw[w] - m) * cs);
-    l += mw[w] * s_part[w][D + 1][jj];
+    l += mw[w] * s_part[w][jj][D + 1];
   }
   if (j >= ncol) return;
-  const int r = j / a.group, hh = h * a.group + j - r * a.group;
+  const int r = row_of(a, j), hh = h * a.group + j - r * a.group;
   const long at = ((long)blockIdx.z * ncol + j) * a.splits + blockIdx.y;
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const int d = ((kw * QT + i) & 3) * 16 + grp * 4;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < KW; ++w)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += mw[w] * s_part[w][d + e][jj];
+    for (int w = 0; w < KW; ++w) y += mw[w] * *(const f32x4*)(s_part[w][jj] + d);
     if (a.splits > 1) *(f32x4*)(a.part + at * D + d) = y;
     else put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + d, y, l, view, r);
   }
@@ -890,7 +888,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   if (tid >= 16) return;
   o = s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid];
   const View view = view_of(a, b, c.state[4 * b], c.state[4 * b + 1]);
-  const int r = j / a.group, hh = h * a.group + j - r * a.group;
+  const int r = row_of(a, j), hh = h * a.group + j - r * a.group;
   put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + d4, o, l, view, r);
 }
 
@@ -931,7 +929,7 @@ Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
   const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
   // workgroups that are resident at once (registers): one round of them
-  const long room = kCUs * (p.qt == 4 ? 2 : 3);
+  const long room = kCUs * (p.qt == 1 ? 4 : p.qt == 2 ? 3 : 2);
   p.splits = (int)max(1L, min(min(room / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
   p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
   return p;
@@ -962,7 +960,7 @@ int attend_args(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void*
       !(scale > 0.f) || !(scale < 1e30f))
     return SVLA_EINVAL;
   if (rows == 0) return SVLA_OK;
-  if ((long)rows * hq > (1L << 24)) return SVLA_EINVAL;
+  if ((long)rows * hq > (1L << 24) || hq / c->n_kv_heads > 255) return SVLA_EINVAL;
   if (!rows_ok(q, ldq, q_bs, hq) || !o || ((uintptr_t)o & 7) || ldo % 4 || o_bs % 4 || ldo < hq * D)
     return SVLA_EINVAL;
   *p = plan_attend(c, rows, hq, window);
@@ -976,6 +974,8 @@ int attend_args(const svla_kv_cache* c, const void* q, int ldq, long q_bs, void*
   a->counts = counts;
   a->rows = rows;
   a->group = hq / c->n_kv_heads;
+  // ceil(2^32 / group): exact while j * group < 2^32 (group 1: no division)
+  a->group_inv = a->group == 1 ? 0u : (unsigned)(((1ULL << 32) + a->group - 1) / a->group);
   a->window = min(window, kMaxPos);
   a->scale_log2 = scale * 1.4426950408889634f;
   a->splits = p->splits;
