@@ -308,8 +308,12 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
     if (nb > 0) {                      // uniform across the workgroup
       start();
       load();
+      const u32x4 k0 = rk[0], k1 = rk[1], v0 = rv[0], v1 = rv[1];
+      load();                          // two blocks on their way
+      const u32x4 k2 = rk[0], k3 = rk[1], v2 = rv[0], v3 = rv[1];
+      rk[0] = k0; rk[1] = k1; rv[0] = v0; rv[1] = v1;
       store();
-      load();
+      rk[0] = k2; rk[1] = k3; rv[0] = v2; rv[1] = v3;
       sync_step();
     }
     for (int blk = 0; blk < nb; ++blk) {

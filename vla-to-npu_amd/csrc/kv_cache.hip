@@ -649,6 +649,9 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
       // all 32 positions are visible to every column of the workgroup
       const bool full = pos0 + TOK - 1 <= qlo && pos0 + TOK <= plim &&
                         (!a.window || pos0 > qhi - a.window || pos0 + TOK <= c.sinks);
+      // (a wave at its matrix products goes before one at its exponentials:
+      // 2 x 1000 rows 35.8 -> 34.7 us, 16 x 65536 tokens 79 -> 76)
+      __builtin_amdgcn_s_setprio(1);
       f32x4 sc[QT][2];
       {
         const bf16x8 k00 = r.template kfrag<0, 0>(), k01 = r.template kfrag<0, 1>();
@@ -727,6 +730,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
           r.vs[3] ^= blk ? w1 : 0u;
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       bf16x8 pf[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -735,6 +739,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
           pf[t][i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t])));
         o[t][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], o[t][4], 0, 0, 0);
       }
+      __builtin_amdgcn_s_setprio(1);
       bf16x8 va, vb;
       r.template vfrags<0>(va, vb);
 #pragma unroll
