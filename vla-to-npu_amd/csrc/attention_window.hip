@@ -2,11 +2,22 @@
 // at position p = q_pos + row sees the keys of positions (p - window, p] and of
 // the first `sinks` positions, of the lens[b] that its sequence has.
 //
-// o = sum_j p_j v_j / sum_j p_j over the visible keys, p_j = 2^(c s_j - c m):
-// one pass over the keys with a running maximum m, rounded probabilities in
-// both sums as in attention_kernel, whose tiles, operand order and LDS ring
-// these are: a workgroup is 64 QT query rows of one head, 16 QT a wave, and
-// streams blocks of 64 keys.
+// o = sum_j p_j v_j / sum_j p_j over the visible keys, p_j = 2^(c s_j - c m), in
+// one pass over the keys, for any reference m (0 but for the second time, see
+// the kernel), with the rounded probabilities in both sums.  Tiles and operand
+// order are attention_kernel's: a workgroup is 64 QT query rows of one head,
+// 16 QT a wave, and goes through the blocks of 64 keys that some row sees.
+//
+// MI355X: 2 x 16384 rows of 15 heads, window 4096, 593 to 610 us (451 GFLOP, 740
+// to 760 TFLOP/s, half of a large library product's 1490).  With 128 rows a
+// workgroup and three waves per SIMD a block of 64 keys and 32 rows takes 1470
+// cycles, of which 36 MFMAs are 576 and the vector instructions 620.  Measured
+// and not kept: the next scores beside the last products in one instruction
+// stream (639 us against 606: two waves per SIMD; on another box 711, of which
+// timing copies without the exponentials took 622 and without staging and
+// barriers 571: no one pipe bounds it), 256 rows (635), 64 rows (722).  8 x 2000 rows of 12 heads, window 500, 57 to 62 us (86 MB, 17.9
+// GFLOP): 10 blocks a workgroup, 4 of them cut by the window's ends; window 64
+// takes 37 us (98 MB).
 #include "attention_tile.h"
 
 namespace {

@@ -33,6 +33,12 @@
 // number of tokens n and the first ring tile still held, lo; lo = kLost marks
 // a sequence whose contents cannot be vouched for (a position that skips
 // ahead was written), until it is written from position 0 again.
+//
+// MI355X, against a large copy's 5.15 TB/s: 4 x 32768 uneven rows of 5 heads
+// written at 4 bits 38 us (159 MB, 4.2 TB/s) and read back 30 (201 MB, 6.7: the
+// L2s hold part); attention of one token over 16 x 65536 tokens of 4 bits 68 + 4
+// (357 MB, 5.2), over 32 contexts of 4096 to 8192 of 8 bits 22.5 + 4 (130 MB,
+// 5.8); 2 x 1000 rows with a window of 2048 28 (15.8 GFLOP, 560 TFLOP/s).
 #include "attention_tile.h"
 
 namespace {
@@ -564,6 +570,12 @@ __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View&
 // from behind the mask, as 0 * NaN), goes over its records once more, following
 // the maximum, and a column then meets only what it sees, NaN blocks apart.
 //
+// What bounds it: one row reads its records at a copy's rate once they are
+// enough to fill the chip; many rows are bound by issue, a record and 64 columns
+// being 36 MFMAs (576 cycles) and ~170 vector instructions (~850 with the 32
+// exponentials), 1370 cycles measured at two waves per SIMD.  Short calls are
+// launch (2 us), the loads of state, then Q and records (1.5), and the joins.
+//
 // PF records are in registers or on their way to them.
 template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2) : 8 / BITS;
 
@@ -867,6 +879,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   const int j = blockIdx.x;
   const int b = blockIdx.y / c.heads, h = blockIdx.y - b * c.heads;
   const long at = ((long)blockIdx.y * ncol + j) * a.splits;
+  // (loads that nothing here decides first: the sequence's state, a lane's part)
+  const View view = view_of(a, b, c.state[4 * b], c.state[4 * b + 1]);
+  const int d4 = (tid & 15) * 4, s0 = tid >> 4;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (s0 < a.splits) o = *(const f32x4*)(a.part + (at + s0) * D + d4);
   // every wave: the weights of the parts and the sum
   float m = -INFINITY;
   for (int s = lane; s < a.splits; s += 64) m = smax(m, a.stat[2 * (at + s)]);
@@ -882,17 +899,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
   __syncthreads();
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int d4 = (tid & 15) * 4;
+  o *= s0 < a.splits ? s_w[s0] : 0.f;
 #pragma unroll 4
-  for (int s = tid >> 4; s < a.splits; s += 16) o += s_w[s] * *(const f32x4*)(a.part + (at + s) * D + d4);
+  for (int s = s0 + 16; s < a.splits; s += 16) o += s_w[s] * *(const f32x4*)(a.part + (at + s) * D + d4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = xor32_sum(xor16_sum(o[i]));
   if (lane < 16) s_o[wave][lane] = o;
   __syncthreads();
   if (tid >= 16) return;
   o = s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid];
-  const View view = view_of(a, b, c.state[4 * b], c.state[4 * b + 1]);
   const int r = row_of(a, j), hh = h * a.group + j - r * a.group;
   put_out(a.o + b * a.o_bs + r * a.ldo + hh * D + d4, o, l, view, r);
 }
@@ -924,17 +939,23 @@ struct Plan {
   dim3 grid;
 };
 
+// QT by columns: 64 columns share the decoding of a record (2 x 1000 rows of 3
+// heads a KV head: 31.5 us against 34.2 with 32, 53 with 16; 32 x 50 rows over
+// 1024 tokens 17.1, 19.0, 33), as long as there are that many.
+//
+// Splits: one round of resident workgroups (16 x 65536 tokens, one row: 79 us
+// with 720 of them, 109 with 240; 1280 in two rounds 83), each with at least 16
+// records, 4 a wave, which are on their way at once.
 Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   Plan p;
   const long ncol = (long)rows * (hq / c->n_kv_heads);
   const long bh = (long)c->batch * c->n_kv_heads;
   p.qt = ncol <= 16 ? 1 : ncol <= 32 ? 2 : 4;
   const long x = (ncol + 16 * p.qt - 1) / (16 * p.qt);
-  // records of a sequence, at most; a wave should have 4 of them
+  // records of a sequence, at most
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
   const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
-  // workgroups that are resident at once (registers): one round of them
-  const long room = kCUs * (p.qt == 1 ? 4 : p.qt == 2 ? 3 : 2);
+  const long room = kCUs * (p.qt == 1 ? 4 : p.qt == 2 ? 3 : 2);    // resident (registers)
   p.splits = (int)max(1L, min(min(room / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
   p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
   return p;
@@ -1095,7 +1116,8 @@ int svla_kv_step_bf16(const svla_kv_cache* c, const void* q, int ldq, long q_bs,
   if (rows > 0 && (!rows_ok(k, ldk, k_bs, c->n_kv_heads) || !rows_ok(v, ldv, v_bs, c->n_kv_heads)))
     return SVLA_EINVAL;
   // One new row, and one workgroup for all the columns of its record: written
-  // on the way (one token after 241 held, write + attention: 11.2 -> ... us)
+  // on the way (one token after 241 held: 6.3 us against 6.0 + 5.2 in two
+  // launches; 32 sequences in windows of 4096: 15.1 + 4.4 against 7.4 + 16.9 + 4.3)
   if (rows != 1 || p.grid.x != 1) {
     const int w = svla_kv_append_bf16(c, k, ldk, k_bs, v, ldv, v_bs, rows, counts, at, stream);
     if (w || rows == 0) return w;

@@ -3,6 +3,7 @@
 * ``smolvla.ops``      -- torch wrappers over the C-ABI of ``libsvla.so``
 * ``smolvla.kernels``  -- the reference's per-kernel harness names
 * ``smolvla.vla``      -- the reference's layer-module signatures
+* ``smolvla.kv_cache`` -- a K/V cache in 8 or 4 bits and the attention over it
 * ``smolvla.pipeline`` -- the full chunk engine (vision -> prefix -> 10 Euler steps)
 """
 
