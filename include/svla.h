@@ -557,8 +557,8 @@ int svla_attention_window_bf16(const void* q, int ldq, long q_bs, const void* k,
  * every token of it was written).  state: [batch][4] int32, set by
  * svla_kv_reset; state[b][0] is n.
  *
- * Values: 32 consecutive values of a row share a power of two 2^E, E in
- * [-110, 126] the smallest for which none saturates (max|x| <= 6 2^E for e2m1,
+ * Values: 32 consecutive values of a row share a power of two 2^E, E the
+ * smallest, -110 at least, for which none saturates (max|x| <= 6 2^E for e2m1,
  * 448 2^E for e4m3); each is the nearest element, ties to the even code.
  * Magnitudes over 1.5 2^127 are stored as that; a block that holds an infinity
  * or a NaN reads as NaN throughout.

@@ -4,9 +4,9 @@
 // Quantisation.  32 consecutive values of a row share a power of two 2^E; an
 // element is the nearest e4m3 or e2m1 number to x / 2^E (ties to the even
 // code: the rounding of v_cvt_scalef32_pk_{fp8,fp4}_bf16).  E is the smallest
-// exponent for which no element saturates, max|x| <= 448 2^E (6 2^E), held
-// within [-110, 126] as the byte E + 127.  With that range every stored value
-// is a normal bf16 number or zero, so reading back and the products below use
+// exponent, -110 at least, for which no element saturates, max|x| <= 448 2^E
+// (6 2^E), held as the byte E + 127.  So every stored value is a normal bf16
+// number or zero, so reading back and the products below use
 // exactly the stored value.  Magnitudes over 1.5 2^127 are stored as that (the
 // next e2m1 step would be infinite).  A block that holds an infinity or a NaN
 // gets the scale byte 0xff and zero codes and reads as NaN throughout.
@@ -118,7 +118,7 @@ template <int BITS> __device__ __forceinline__ int scale_byte(unsigned top) {
   // top = 2^(e-127) (1 + m/128): the largest element is 1.5 2^2 (1.75 2^8)
   const int e = (int)(top >> 7), m = (int)(top & 127);
   const int s = BITS == 4 ? e - 2 + (m > 0x40) : e - 8 + (m > 0x60);
-  return min(max(s, 17), 253);
+  return max(s, 17);
 }
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -132,7 +132,7 @@ template <int BITS> __device__ __forceinline__ u32x2 encode8(u32x4 x, int byte) 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     unsigned w = x[i];
-    if (byte == 253 || (BITS == 8 && byte >= 246)) {      // clamp to +-1.5 2^127
+    if (BITS == 8 && byte == 246) {      // +-1.5 2^127 (e2m1 saturates there itself)
       unsigned a = w & 0x7fff, b = (w >> 16) & 0x7fff;
       a = min(a, 0x7f40u) | (w & 0x8000u);
       b = min(b, 0x7f40u) | ((w >> 16) & 0x8000u);
@@ -570,6 +570,12 @@ __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View&
 // from behind the mask, as 0 * NaN), goes over its records once more, following
 // the maximum, and a column then meets only what it sees, NaN blocks apart.
 //
+// Up to 64 columns a KV head (QT < 4) the probabilities go into the products as
+// bf16 and a bf16 remainder: what they would be off by, 2^-9 in the mean square,
+// is as much as the output's own rounding.  Such calls read or wait, so it is
+// free there; with more columns the products are what costs, and the
+// probabilities are rounded once, as in attention_kernel.
+//
 // What bounds it: one row reads its records at a copy's rate once they are
 // enough to fill the chip; many rows are bound by issue, a record and 64 columns
 // being 36 MFMAs (576 cycles) and ~170 vector instructions (~850 with the 32
@@ -583,6 +589,7 @@ template <int BITS, int QT> constexpr int kAhead = QT == 1 ? (BITS == 4 ? 3 : 2)
 template <int BITS, int QT, bool NEW>
 __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs a) {
   constexpr int PF = kAhead<BITS, QT>, KW = 4, LD = D + 4;
+  constexpr bool TWO = QT < 4;                     // probabilities in two bf16 terms
   // per wave and column: 64 depths, reference, sum
   __shared__ __attribute__((aligned(16))) float s_part[KW][16 * QT][LD];
   const Cache& c = a.c;
@@ -743,28 +750,33 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      bf16x8 pf[QT];
+      bf16x8 pf[QT], pl[TWO ? QT : 1];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          pf[t][i] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t])));
+        for (int i = 0; i < 8; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], cs, m_off[t]));
+          pf[t][i] = f2bf(e);
+          if constexpr (TWO) pl[t][i] = f2bf(e - bf2f(pf[t][i]));
+        }
         o[t][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[t], o[t][4], 0, 0, 0);
+        if constexpr (TWO) o[t][4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pl[t], o[t][4], 0, 0, 0);
       }
       __builtin_amdgcn_s_setprio(1);
       bf16x8 va, vb;
+      auto product = [&](int td, bf16x8 vf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t], o[t][td], 0, 0, 0);
+          if constexpr (TWO) o[t][td] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[t], o[t][td], 0, 0, 0);
+        }
+      };
       r.template vfrags<0>(va, vb);
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        o[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[t], o[t][0], 0, 0, 0);
-        o[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pf[t], o[t][1], 0, 0, 0);
-      }
+      product(0, va);
+      product(1, vb);
       r.template vfrags<1>(va, vb);
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        o[t][2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pf[t], o[t][2], 0, 0, 0);
-        o[t][3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pf[t], o[t][3], 0, 0, 0);
-      }
+      product(2, va);
+      product(3, vb);
     };
     // the newest record, where the new row goes: its wave takes it first
     const bool newest = NEW && t1 == total && kw == ((total - 1 - t0) & (KW - 1));
@@ -941,7 +953,7 @@ struct Plan {
 
 // QT by columns: 64 columns share the decoding of a record (2 x 1000 rows of 3
 // heads a KV head: 31.5 us against 34.2 with 32, 53 with 16; 32 x 50 rows over
-// 1024 tokens 17.1, 19.0, 33), as long as there are that many.
+// 1024 tokens 17.1, 19.0, 33), as long as there are more than that.
 //
 // Splits: one round of resident workgroups (16 x 65536 tokens, one row: 79 us
 // with 720 of them, 109 with 240; 1280 in two rounds 83), each with at least 16
@@ -950,7 +962,7 @@ Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   Plan p;
   const long ncol = (long)rows * (hq / c->n_kv_heads);
   const long bh = (long)c->batch * c->n_kv_heads;
-  p.qt = ncol <= 16 ? 1 : ncol <= 32 ? 2 : 4;
+  p.qt = ncol <= 16 ? 1 : ncol <= 64 ? 2 : 4;
   const long x = (ncol + 16 * p.qt - 1) / (16 * p.qt);
   // records of a sequence, at most
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
@@ -969,8 +981,7 @@ template <int BITS>
 void launch_attend(const Plan& p, const AttendArgs& a, hipStream_t s) {
   if (a.k) {
     if (p.qt == 1) hipLaunchKernelGGL((attend_kernel<BITS, 1, true>), p.grid, dim3(256), 0, s, a);
-    else if (p.qt == 2) hipLaunchKernelGGL((attend_kernel<BITS, 2, true>), p.grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attend_kernel<BITS, 4, true>), p.grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attend_kernel<BITS, 2, true>), p.grid, dim3(256), 0, s, a);   // (one workgroup's columns: at most 32)
   } else {
     if (p.qt == 1) hipLaunchKernelGGL((attend_kernel<BITS, 1, false>), p.grid, dim3(256), 0, s, a);
     else if (p.qt == 2) hipLaunchKernelGGL((attend_kernel<BITS, 2, false>), p.grid, dim3(256), 0, s, a);

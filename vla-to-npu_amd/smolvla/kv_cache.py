@@ -142,8 +142,9 @@ class KVCache:
     def _ints(self, name, t):
         if t is None:
             return None
-        if not (torch.is_tensor(t) and t.dtype is torch.int32 and t.shape == (self.batch,)
-                and t.is_contiguous() and t.device == self.device):
+        if not (torch.is_tensor(t) and t.dtype is torch.int32 and t.dim() == 1
+                and t.shape[0] == self.batch and (t.stride(0) == 1 or self.batch == 1)
+                and t.device == self.device):
             raise ValueError(f"{name}: contiguous int32 [{self.batch}] tensor on {self.device} "
                              "expected")
         return t.data_ptr()
