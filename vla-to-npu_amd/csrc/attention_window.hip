@@ -13,7 +13,7 @@
 // workgroup and three waves per SIMD a block of 64 keys and 32 rows takes 1470
 // cycles, of which 36 MFMAs are 576 and the vector instructions 620.  Measured
 // and not kept: the next scores beside the last products in one instruction
-// stream (639 us against 606: two waves per SIMD; on another box 711, of which
+// stream (639 us against 606: two waves per SIMD; in another run 711, of which
 // timing copies without the exponentials took 622 and without staging and
 // barriers 571: no one pipe bounds it), 256 rows (635), 64 rows (722).  8 x 2000 rows of 12 heads, window 500, 57 to 62 us (86 MB, 17.9
 // GFLOP): 10 blocks a workgroup, 4 of them cut by the window's ends; window 64

@@ -36,9 +36,9 @@
 //
 // MI355X, against a large copy's 5.15 TB/s: 4 x 32768 uneven rows of 5 heads
 // written at 4 bits 38 us (159 MB, 4.2 TB/s) and read back 30 (201 MB, 6.7: the
-// L2s hold part); attention of one token over 16 x 65536 tokens of 4 bits 68 + 4
-// (357 MB, 5.2), over 32 contexts of 4096 to 8192 of 8 bits 22.5 + 4 (130 MB,
-// 5.8); 2 x 1000 rows with a window of 2048 28 (15.8 GFLOP, 560 TFLOP/s).
+// L2s hold part); attention of one token over 16 x 65536 tokens of 4 bits 73 + 4
+// (357 MB, 4.9), over 32 contexts of 4096 to 8192 of 8 bits 23 + 4 (130 MB, 5.6);
+// 2 x 1000 rows with a window of 2048 28 (15.8 GFLOP, 560 TFLOP/s).
 #include "attention_tile.h"
 
 namespace {
@@ -572,8 +572,8 @@ __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View&
 //
 // Up to 64 columns a KV head (QT < 4) the probabilities go into the products as
 // bf16 and a bf16 remainder: what they would be off by, 2^-9 in the mean square,
-// is as much as the output's own rounding.  Such calls read or wait, so it is
-// free there; with more columns the products are what costs, and the
+// is as much as the output's own rounding.  Such calls read or wait, so it costs
+// little there (16 x 65536 tokens 70 -> 74 us, 8 bits nothing); with more columns the products are what costs, and the
 // probabilities are rounded once, as in attention_kernel.
 //
 // What bounds it: one row reads its records at a copy's rate once they are
@@ -955,9 +955,10 @@ struct Plan {
 // heads a KV head: 31.5 us against 34.2 with 32, 53 with 16; 32 x 50 rows over
 // 1024 tokens 17.1, 19.0, 33), as long as there are more than that.
 //
-// Splits: one round of resident workgroups (16 x 65536 tokens, one row: 79 us
-// with 720 of them, 109 with 240; 1280 in two rounds 83), each with at least 16
-// records, 4 a wave, which are on their way at once.
+// Splits: one round of three workgroups a CU, two of 64 columns (16 x 65536
+// tokens, one row: 79 us with 720 workgroups, 109 with 240, 80 with 960; one
+// sequence of 100003: 14.8 us with 154, 15.8 with 196, whose parts cost the join
+// more), each with at least 16 records, 4 a wave, which are on their way at once.
 Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   Plan p;
   const long ncol = (long)rows * (hq / c->n_kv_heads);
@@ -967,7 +968,7 @@ Plan plan_attend(const svla_kv_cache* c, int rows, int hq, int window) {
   // records of a sequence, at most
   const long ring = window ? min((long)c->ring, (long)window + rows + 2 * TOK) : (long)c->ring;
   const long tiles = ring / TOK + (c->sinks + TOK - 1) / TOK;
-  const long room = kCUs * (p.qt == 1 ? 4 : p.qt == 2 ? 3 : 2);    // resident (registers)
+  const long room = kCUs * (p.qt == 4 ? 2 : 3);
   p.splits = (int)max(1L, min(min(room / (x * bh), (tiles + 15) / 16), (long)kMaxSplits));
   p.grid = dim3((unsigned)x, (unsigned)p.splits, (unsigned)bh);
   return p;
