@@ -340,6 +340,22 @@ def test_a_first_score_far_below_the_others():
         close(cache.attend(q, 2, scale=2.0), want.attend(q, 2, scale=2.0))
 
 
+@pytest.mark.parametrize("level", [-12.0, -25.0, -60.0, -2000.0])
+def test_scores_far_below_zero_and_tiny_values(level):
+    """Every score around ``level``: sums of exp(s) that are small or zero, with
+    values that a product with them would lose."""
+    g = gen(23)
+    for rows in (1, 24, 90):
+        cache, want = KVCache(1, 1, max_len=200, fmt="mxfp8"), ref.CacheRef(1, 1, "mxfp8")
+        k, v = rand(g, 1, 200, 64, scale=0.05), rand(g, 1, 200, 64, scale=2.0 ** -80)
+        k[..., 0], k[..., 32] = 1.0, 1.0
+        q = rand(g, 1, rows, 128)
+        q.view(1, rows, 2, 64)[..., 0] = level * 8
+        cache.append(k, v)
+        want.append(k, v)
+        close(cache.attend(q, 2), want.attend(q, 2))
+
+
 def test_time_before_batch_and_in_place():
     """[T, B, .] tensors as [B, T, .] views, and the output over the queries."""
     g = gen(22)

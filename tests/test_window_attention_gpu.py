@@ -81,6 +81,18 @@ def test_scores_that_outgrow_the_first_ones(n):
     check(q, k, v, 2, 1, 300, 1)
 
 
+@pytest.mark.parametrize("level", [-12.0, -25.0, -60.0, -2000.0])
+def test_scores_far_below_zero_and_tiny_values(level):
+    """Every score around ``level``: sums of exp(s) that are small or zero, with
+    values that a product with them would lose."""
+    g = gen(13)
+    n = 150
+    q, k, v = rand(g, 1, n, 128), rand(g, 1, n, 64, scale=0.05), rand(g, 1, n, 64, scale=2.0 ** -80)
+    k[..., 0] = 1.0
+    q.view(1, n, 2, 64)[..., 0] = level * 8
+    check(q, k, v, 2, 1, 60, 2)
+
+
 def test_uneven_lengths_and_views():
     """Padded sequences (one empty), fused projection views, a strided output
     whose other columns stay; rows past their window of a short sequence see

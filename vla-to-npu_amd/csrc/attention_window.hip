@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
   // Softmax needs no maximum where exp(s) itself neither over- nor underflows:
   // any reference gives the same quotient, and bf16 keeps fp32's range.  So the
   // first time over the keys takes the reference 0.  Where a row's sum leaves
-  // [2^-60, 2^100], or an output 2^100 (also by infinities and NaNs, even from
+  // [2^-40, 2^100], or an output 2^100 (also by infinities and NaNs, even from
   // behind the mask, as 0 * NaN), the workgroup goes over its keys once more,
   // following the maximum, and a row then meets only what it sees, infinities
   // and NaNs apart.
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256, QT == 2 ? 3 : 4) void window_kernel(WindowArgs
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = smax(top, fabsf(o[qt][t][i]));
       const bool sees_some = last[qt] > max(before[qt], -1) || (p.sinks > 0 && last[qt] >= 0);
-      bad |= sees_some && !(top < 0x1p100f && o[qt][4][0] >= 0x1p-60f);
+      bad |= sees_some && !(top < 0x1p100f && o[qt][4][0] >= 0x1p-40f);
     }
     if (track || !__syncthreads_or(bad && qw < p.sq)) break;
     track = 1;

@@ -566,15 +566,16 @@ __device__ __forceinline__ void put_out(bf16* out, f32x4 o, float l, const View&
 // Softmax needs no maximum where exp(s) itself neither over- nor underflows: any
 // reference gives the same quotient, and bf16 keeps fp32's range.  So the first
 // time over the records takes the reference 0.  A wave of which a column's sum
-// leaves [2^-60, 2^100], or an output 2^100 (also by infinities and NaNs, even
+// leaves [2^-40, 2^100], or an output 2^100 (also by infinities and NaNs, even
 // from behind the mask, as 0 * NaN), goes over its records once more, following
 // the maximum, and a column then meets only what it sees, NaN blocks apart.
 //
 // Up to 64 columns a KV head (QT < 4) the probabilities go into the products as
 // bf16 and a bf16 remainder: what they would be off by, 2^-9 in the mean square,
 // is as much as the output's own rounding.  Such calls read or wait, so it costs
-// little there (16 x 65536 tokens 70 -> 74 us, 8 bits nothing); with more columns the products are what costs, and the
-// probabilities are rounded once, as in attention_kernel.
+// little there (16 x 65536 tokens 70 -> 74 us, 8 bits nothing); with more columns
+// the products are what costs, and the probabilities are rounded once, as in
+// attention_kernel.
 //
 // What bounds it: one row reads its records at a copy's rate once they are
 // enough to fill the chip; many rows are bound by issue, a record and 64 columns
@@ -650,7 +651,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
     const int from = t0 + kw;
     const uint8_t* base = c.data + record(c, b, h, 0) * kRec<BITS>;
     // record of place ti in the list (past the end: the last one)
-    int at_u = u0 % c.ring_tiles;
+    const int at_u = u0 % c.ring_tiles;
     auto addr = [&](int ti) {
       ti = min(ti, t1 - 1);
       int u = ti;
@@ -660,7 +661,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
       }
       return base + (long)u * kRec<BITS>;
     };
-    // One record.  FOLLOW: the second time.
+    // One record.  FOLLOW: the second time over them, see above.
     auto step = [&](auto FOLLOW, Rec<BITS>& r, int ti) __attribute__((always_inline)) {
       const bool sink = ti < ns;
       const int pos0 = sink ? ti * TOK : c.sinks + (u0 + ti - ns) * TOK;
@@ -812,7 +813,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 3) void attend_kernel(AttendArgs
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = smax(top, fabsf(o[t][i][e]));
-        bad |= qpos[t] >= 0 && !(top < 0x1p100f && o[t][4][0] >= 0x1p-60f);
+        bad |= qpos[t] >= 0 && !(top < 0x1p100f && o[t][4][0] >= 0x1p-40f);
         m_run[t] = 0.f;
       }
       if (__builtin_amdgcn_ballot_w64(bad)) {
